@@ -385,6 +385,127 @@ int pt_s4_head_grad_f32(const float* x, const float* gy, const float* w, float* 
                         int B, int H, int L, int outputs, void* stream);
 
 /*
+ * A selective state space block, channels last: the short causal depthwise
+ * convolution, the selective scan, and the norms around them. Activations are
+ * FP32 or BF16 (dtype PT_F32 or PT_BF16, PT_ERR_CONFIG otherwise), computed on
+ * in FP32 and rounded once; weights, scan states and parameter gradients are
+ * FP32. Rows hold contiguous channels; strides of inputs are in elements, so
+ * that a slice of a projection's output can be passed as it is. Outputs are
+ * contiguous. Pointers need their type's alignment; 16-byte aligned ones with
+ * strides and channels in multiples of 16 bytes take wide loads. Offsets are
+ * 64-bit: only each size is limited (PT_ERR_SHAPE), and a launch to 2^32
+ * lanes. B (or rows) = 0 launches nothing but zero parameter gradients.
+ * Parameter gradients are added in a fixed order. `lengths` [B] (NULL: all L)
+ * are the tokens of each sequence, clamped to [0, L]; what lies past them is
+ * not used, and outputs and gradients there are 0.
+ */
+#define PT_F32 0
+#define PT_BF16 1
+
+/*
+ * Causal convolution, 1 <= K <= 8, w [H, K]:
+ *   p[b,t,h] = bias[h] + sum_j w[h,j] x[b,t-(K-1)+j,h],  y = silu ? silu(p) : p
+ * with the tokens before the first from state [B, K-1, H] (NULL: 0), in x's
+ * type, oldest first; state_out (NULL: none) gets the last K-1 tokens of each
+ * sequence. bias may be NULL. _bwd gives the gradients of x, w, bias (NULL:
+ * skipped) and state (NULL: skipped) from gy [B, L, H] and the final state's
+ * gradient gstate_out (NULL: 0).
+ * _step takes one token x [B, H] of each of B sequences, whose states are rows
+ * slots[b] (NULL: row b) of a pool [pool, K-1, H] and shift in place. A slot
+ * outside [0, pool) marks a row without a sequence: its y is 0. Slots must
+ * differ from each other.
+ */
+int pt_causal_conv_fwd(int dtype, const void* x, long long x_batch, long long x_row,
+                       const float* w, const float* bias, const void* state,
+                       const int* lengths, void* y, void* state_out, int B, int L, int H,
+                       int K, int silu, void* stream);
+int pt_causal_conv_bwd_workspace_bytes(int dtype, int B, int L, int H, int K, size_t* bytes);
+int pt_causal_conv_bwd(int dtype, const void* x, long long x_batch, long long x_row,
+                       const float* w, const float* bias, const void* state,
+                       const int* lengths, const void* gy, const void* gstate_out, void* gx,
+                       float* gw, float* gbias, void* gstate, void* workspace,
+                       size_t workspace_bytes, int B, int L, int H, int K, int silu,
+                       void* stream);
+int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* w,
+                        const float* bias, void* state, const int* slots, void* y, int B,
+                        int H, int K, int pool, int silu, void* stream);
+
+/*
+ * Selective scan, 1 <= N <= 64 states, G groups of H / G channels that share
+ * their B and C:
+ *   v = dt + dt_bias,  delta = softplus ? softplus(v) : v
+ *   s[n] = exp(delta A[h,n]) s[n] + delta x B[b,t,g,n]
+ *   y[b,t,h] = sum_n C[b,t,g,n] s[n] + D[h] x[b,t,h]
+ * x, dt [B, L, H]; B, C [B, L, G, N] with contiguous states (b_group: between
+ * groups); A [H, N]; D and dt_bias [H] or NULL (0); the first state [B, H, N]
+ * or NULL (0). delta must not be negative with A positive beyond FP32's range.
+ * _sizes gives the bytes of the workspaces and of `saved`, which _fwd fills
+ * where not NULL (the state before every 16 tokens) and _bwd takes with the
+ * same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;
+ * gd, gdt_bias and gstate are skipped where NULL; gb, gc are [B, L, G, N].
+ * _step: one token, x and dt [B, H] and B, C [B, G, N] with the batch strides
+ * (row strides and L are not read); states [pool, H, N] and slots as in
+ * pt_causal_conv_step.
+ */
+typedef struct pt_scan_inputs {
+  const void *x, *dt, *b, *c;
+  const float *a, *d, *dt_bias, *state;
+  const int* lengths;
+  long long x_batch, x_row, dt_batch, dt_row, b_batch, b_row, b_group, c_batch, c_row, c_group;
+  int dtype, B, L, H, N, G, softplus;
+} pt_scan_inputs;
+
+int pt_selective_scan_sizes(const pt_scan_inputs* in, size_t* fwd_workspace, size_t* saved,
+                            size_t* bwd_workspace);
+int pt_selective_scan_fwd(const pt_scan_inputs* in, void* y, float* state_out, float* saved,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float* saved,
+                          const float* gstate_out, void* gx, void* gdt, float* ga, void* gb,
+                          void* gc, float* gd, float* gdt_bias, float* gstate, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int pt_selective_scan_step(const pt_scan_inputs* in, float* state, const int* slots, int pool,
+                           void* y, void* stream);
+
+/*
+ * Gated norm over groups of H / groups <= 16384 channels:
+ *   u = x silu(gate),  y = u rsqrt(mean u^2 + eps) w
+ * rstd [rows, groups] (NULL: none) is what _bwd takes.
+ */
+int pt_gated_norm_fwd(int dtype, const void* x, long long x_row, const void* gate,
+                      long long gate_row, const float* w, void* y, float* rstd, long long rows,
+                      int H, int groups, float eps, void* stream);
+int pt_gated_norm_bwd_workspace_bytes(int dtype, long long rows, int H, int groups,
+                                      size_t* bytes);
+int pt_gated_norm_bwd(int dtype, const void* x, long long x_row, const void* gate,
+                      long long gate_row, const float* w, const float* rstd, const void* gy,
+                      void* gx, void* ggate, float* gw, void* workspace,
+                      size_t workspace_bytes, long long rows, int H, int groups, void* stream);
+
+/*
+ * Residual norm, H <= 16384: the end of one block and the start of the next,
+ *   f = x, or with post_w  x rsqrt(mean x^2 + eps) post_w
+ *   sum = residual + scale f,  y = sum rsqrt(mean sum^2 + eps) w
+ * residual (NULL: 0) and sum are res_dtype: x's type or FP32. post_w and scale
+ * [H] may be NULL. y is computed on the sum before its rounding; rstd and
+ * rstd_x [rows] (NULL: none; rstd_x with post_w only) are what _bwd takes. In
+ * _bwd gsum (NULL: 0) is the sum's gradient, gresidual may be NULL, and
+ * gparams holds the gradients of w, of scale and of post_w, [1 to 3, H], those
+ * that are there; `sums` counts them.
+ */
+int pt_residual_norm_fwd(int dtype, int res_dtype, const void* x, long long x_row,
+                         const void* residual, long long res_row, const float* post_w,
+                         const float* scale, const float* w, void* y, void* sum, float* rstd,
+                         float* rstd_x, long long rows, int H, float eps, void* stream);
+int pt_residual_norm_bwd_workspace_bytes(int dtype, long long rows, int H, int sums,
+                                         size_t* bytes);
+int pt_residual_norm_bwd(int dtype, int res_dtype, const void* x, long long x_row,
+                         const void* residual, long long res_row, const float* post_w,
+                         const float* scale, const float* w, const float* rstd,
+                         const float* rstd_x, const void* gy, const void* gsum, void* gx,
+                         void* gresidual, float* gparams, void* workspace,
+                         size_t workspace_bytes, long long rows, int H, void* stream);
+
+/*
  * Compiled resources of the kernel that serves (L, K) for `kernel_id`
  * (PT_KERNEL_*), as hipFuncGetAttributes reports them on the current device:
  * registers per lane, static LDS bytes, scratch (private) bytes per lane and

@@ -48,11 +48,32 @@ PT_KERNEL_DX_STREAM = 8
 PT_KERNEL_FWD_CG16 = 9
 PT_KERNEL_DX_CG16 = 10
 
+# activation types of the selective state space block
+PT_F32 = 0
+PT_BF16 = 1
+
 # Every symbol include/pathtile_hip.h declares, with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _ip = ctypes.POINTER(ctypes.c_int)
 _szp = ctypes.POINTER(ctypes.c_size_t)
+_ll = ctypes.c_longlong
+_f = ctypes.c_float
+_sz = ctypes.c_size_t
+
+
+class ScanInputs(ctypes.Structure):
+    """pt_scan_inputs."""
+
+    _fields_ = (
+        [(n, _vp) for n in ("x", "dt", "b", "c", "a", "d", "dt_bias", "state", "lengths")]
+        + [(n, _ll) for n in ("x_batch", "x_row", "dt_batch", "dt_row", "b_batch", "b_row",
+                              "b_group", "c_batch", "c_row", "c_group")]
+        + [(n, _i) for n in ("dtype", "B", "L", "H", "N", "G", "softplus")]
+    )
+
+
+_scan = ctypes.POINTER(ScanInputs)
 SIGNATURES = {
     "pt_abi_version": (_i, []),
     "pt_status_string": (ctypes.c_char_p, [_i]),
@@ -105,6 +126,30 @@ SIGNATURES = {
     "pt_s4_head_f32": (_i, [_vp] * 4 + [_i] * 4 + [_vp]),
     "pt_s4_head_grad_workspace_bytes": (_i, [_i] * 4 + [_szp]),
     "pt_s4_head_grad_f32": (_i, [_vp] * 7 + [ctypes.c_size_t] + [_i] * 4 + [_vp]),
+    "pt_causal_conv_fwd": (_i, [_i, _vp, _ll, _ll] + [_vp] * 6 + [_i] * 5 + [_vp]),
+    "pt_causal_conv_bwd_workspace_bytes": (_i, [_i] * 5 + [_szp]),
+    "pt_causal_conv_bwd": (
+        _i, [_i, _vp, _ll, _ll] + [_vp] * 11 + [_sz] + [_i] * 5 + [_vp]
+    ),
+    "pt_causal_conv_step": (_i, [_i, _vp, _ll] + [_vp] * 5 + [_i] * 5 + [_vp]),
+    "pt_selective_scan_sizes": (_i, [_scan] + [_szp] * 3),
+    "pt_selective_scan_fwd": (_i, [_scan] + [_vp] * 4 + [_sz, _vp]),
+    "pt_selective_scan_bwd": (_i, [_scan] + [_vp] * 12 + [_sz, _vp]),
+    "pt_selective_scan_step": (_i, [_scan, _vp, _vp, _i, _vp, _vp]),
+    "pt_gated_norm_fwd": (
+        _i, [_i, _vp, _ll, _vp, _ll] + [_vp] * 3 + [_ll, _i, _i, _f, _vp]
+    ),
+    "pt_gated_norm_bwd_workspace_bytes": (_i, [_i, _ll, _i, _i, _szp]),
+    "pt_gated_norm_bwd": (
+        _i, [_i, _vp, _ll, _vp, _ll] + [_vp] * 7 + [_sz, _ll, _i, _i, _vp]
+    ),
+    "pt_residual_norm_fwd": (
+        _i, [_i, _i, _vp, _ll, _vp, _ll] + [_vp] * 7 + [_ll, _i, _f, _vp]
+    ),
+    "pt_residual_norm_bwd_workspace_bytes": (_i, [_i, _ll, _i, _i, _szp]),
+    "pt_residual_norm_bwd": (
+        _i, [_i, _i, _vp, _ll, _vp, _ll] + [_vp] * 11 + [_sz, _ll, _i, _vp]
+    ),
     "pt_kernel_attributes": (_i, [_i, _i, _i, _ip, _ip, _ip, _ip]),
     "pt_dynamic_lds_bytes": (_i, [_i, _i, _i, _i, _ip]),
 }

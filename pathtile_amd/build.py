@@ -48,6 +48,11 @@ SOURCES = [
     "inst_s4_tail_fwd.hip",
     "inst_s4_tail_bwd.hip",
     "inst_s4_dw.hip",
+    "ssm_conv.hip",
+    "ssm_norm.hip",
+    "ssm_scan.hip",
+    "inst_ssm_scan_fwd.hip",
+    "inst_ssm_scan_bwd.hip",
 ]
 INCLUDE = ROOT / "include"
 BUILD_DIR = PKG / "_build"

@@ -1,0 +1,92 @@
+// ssm_common.hpp — what the kernels of the selective state space block share:
+// loads and stores of FP32 and BF16 activations, and the scalar functions.
+// Activations are FP32 or BF16 and are computed on in FP32; an output is
+// rounded to its type once, as it is stored.
+
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace pt {
+
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+using f4v = __attribute__((ext_vector_type(4))) float;
+using u4v = __attribute__((ext_vector_type(4))) uint32_t;
+using u2v = __attribute__((ext_vector_type(2))) uint32_t;
+
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)lo) |
+         (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)hi) << 16;
+}
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
+
+// V consecutive values, p aligned to all of them (to 16 bytes from there on).
+template <int V>
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[V]) {
+  static_assert(V % 4 == 0, "whole pieces of 16 bytes");
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    const f4v q = *reinterpret_cast<const f4v*>(p + i);
+    v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+  }
+}
+template <int V>
+__device__ __forceinline__ void load_vec(const __bf16* p, float (&v)[V]) {
+  static_assert(V == 4 || V % 8 == 0, "8 bytes or whole pieces of 16");
+  if constexpr (V == 4) {
+    const u2v q = *reinterpret_cast<const u2v*>(p);
+    v[0] = bf16_lo(q.x), v[1] = bf16_hi(q.x), v[2] = bf16_lo(q.y), v[3] = bf16_hi(q.y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 8) {
+      const u4v q = *reinterpret_cast<const u4v*>(p + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + 2 * j] = bf16_lo(q[j]), v[i + 2 * j + 1] = bf16_hi(q[j]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 4)
+    *reinterpret_cast<f4v*>(p + i) = f4v{v[i], v[i + 1], v[i + 2], v[i + 3]};
+}
+template <int V>
+__device__ __forceinline__ void store_vec(__bf16* p, const float (&v)[V]) {
+  if constexpr (V == 4) {
+    *reinterpret_cast<u2v*>(p) = u2v{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 8) {
+      u4v q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = bf16_pair(v[i + 2 * j], v[i + 2 * j + 1]);
+      *reinterpret_cast<u4v*>(p + i) = q;
+    }
+  }
+}
+
+// exp(v): the exponent in two terms, so that its rounding stays below 2^-24 of
+// the result for any |v|; a result below 2^-126 is 0.
+__device__ __forceinline__ float exp_f32(float v) {
+  return __builtin_amdgcn_exp2f(fmaf(v, 1.44269502162933349609375f, v * 1.92596303e-08f));
+}
+__device__ __forceinline__ float sigmoid_f32(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v));
+}
+// d/dp of p sigmoid(p), from sig = sigmoid(p)
+__device__ __forceinline__ float silu_grad_f32(float p, float sig) {
+  return sig * fmaf(p, 1.0f - sig, 1.0f);
+}
+
+}  // namespace pt

@@ -1,0 +1,225 @@
+// ssm_norm.hip — entry points of the norms around a selective state space block.
+
+#include "ssm_host.hpp"
+#include "ssm_norm.hpp"
+
+namespace pt {
+
+// How a row is held: TPR lanes of E values, vectors of eight or single values.
+struct NormForm {
+  int tpr, e;
+  bool vec;
+};
+
+// A wave up to 1024 channels, four up to 4096, sixteen up to 16384, with 8 or
+// 16 values a lane.
+static NormForm norm_form(int h, bool vec) {
+  NormForm f = {h <= 1024 ? 64 : h <= 4096 ? 256 : 1024, 16, vec};
+  if (f.tpr * 8 >= h) f.e = 8;
+  return f;
+}
+
+template <template <int, int, bool> class F>
+static const void* norm_fn(const NormForm& f) {
+  if (f.vec) {
+    if (f.tpr == 64) return f.e == 8 ? F<8, 64, true>::fn() : F<16, 64, true>::fn();
+    if (f.tpr == 256) return f.e == 8 ? F<8, 256, true>::fn() : F<16, 256, true>::fn();
+    return f.e == 8 ? F<8, 1024, true>::fn() : F<16, 1024, true>::fn();
+  }
+  if (f.tpr == 64) return f.e == 8 ? F<8, 64, false>::fn() : F<16, 64, false>::fn();
+  if (f.tpr == 256) return f.e == 8 ? F<8, 256, false>::fn() : F<16, 256, false>::fn();
+  return f.e == 8 ? F<8, 1024, false>::fn() : F<16, 1024, false>::fn();
+}
+
+template <typename T>
+struct Gated {
+  template <int E, int TPR, bool VEC>
+  struct Fwd {
+    static const void* fn() { return (const void*)&gated_fwd_kernel<T, E, TPR, VEC>; }
+  };
+  template <int E, int TPR, bool VEC>
+  struct Bwd {
+    static const void* fn() { return (const void*)&gated_bwd_kernel<T, E, TPR, VEC>; }
+  };
+};
+template <typename T, typename RT>
+struct Residual {
+  template <int E, int TPR, bool VEC>
+  struct Fwd {
+    static const void* fn() { return (const void*)&residual_fwd_kernel<T, RT, E, TPR, VEC>; }
+  };
+  template <int E, int TPR, bool VEC>
+  struct Bwd {
+    static const void* fn() { return (const void*)&residual_bwd_kernel<T, RT, E, TPR, VEC>; }
+  };
+};
+
+static bool known(int dtype) { return dtype == PT_F32 || dtype == PT_BF16; }
+
+static bool all16(const void* const* p, int n) {
+  for (int i = 0; i < n; ++i)
+    if (!ssm_aligned(p[i], 16)) return false;
+  return true;
+}
+
+// Workgroups of a backward pass: four to a CU where a row takes four waves or
+// fewer, one where it takes sixteen, and no more than there are rows; a
+// multiple of what keeps a lane's rows in one group.
+static long long norm_grid(long long rows, const NormForm& f, int groups) {
+  const int per = norm_threads(f.tpr) / f.tpr;
+  long long n = f.tpr == 1024 ? 256 : 1024;
+  if (n > ssm_ceil(rows, per)) n = ssm_ceil(rows, per);
+  int g = groups, p = per;
+  while (p) { const int r = g % p; g = p; p = r; }  // g = gcd(groups, per)
+  const int q = groups / g;
+  return ssm_ceil(n, q) * q;
+}
+
+static int check_gated(int dtype, long long rows, int H, int groups) {
+  if (!known(dtype)) return PT_ERR_CONFIG;
+  if (rows < 0 || H < 1 || groups < 1 || H % groups || H / groups > kNormMaxH) return PT_ERR_SHAPE;
+  return PT_OK;
+}
+static int check_residual(int dtype, int res_dtype, long long rows, int H) {
+  if (!known(dtype) || (res_dtype != dtype && res_dtype != PT_F32)) return PT_ERR_CONFIG;
+  if (rows < 0 || H < 1 || H > kNormMaxH) return PT_ERR_SHAPE;
+  return PT_OK;
+}
+
+// The parts' layout must not depend on alignment: the same workspace serves.
+static long long gated_parts(long long rows, int H, int groups) {
+  const NormForm f = norm_form(H / groups, true);
+  return norm_grid(rows * groups, f, groups) * (norm_threads(f.tpr) / f.tpr) / groups;
+}
+static long long residual_parts(long long rows, int H) {
+  const NormForm f = norm_form(H, true);
+  return norm_grid(rows, f, 1) * (norm_threads(f.tpr) / f.tpr);
+}
+
+static int sum_columns(const float* part, float* out, long long parts, int cols, void* stream) {
+  void* args[] = {&part, &out, &parts, &cols};
+  return ssm_launch((const void*)&column_sum_kernel, ssm_ceil(cols, 64), 256, stream, args);
+}
+
+}  // namespace pt
+
+extern "C" {
+
+int pt_gated_norm_fwd(int dtype, const void* x, long long x_row, const void* gate,
+                      long long gate_row, const float* w, void* y, float* rstd, long long rows,
+                      int H, int groups, float eps, void* stream) {
+  const int st = pt::check_gated(dtype, rows, H, groups);
+  if (st != PT_OK) return st;
+  if (rows == 0) return PT_OK;
+  if (!x || !gate || !w || !y) return PT_ERR_NULL;
+  const int hg = H / groups;
+  const void* ptrs[] = {x, gate, w, y};
+  const pt::NormForm f = pt::norm_form(
+      hg, hg % 8 == 0 && x_row % 8 == 0 && gate_row % 8 == 0 && pt::all16(ptrs, 4));
+  pt::NormArgs a = {x, gate, nullptr, w, nullptr, nullptr, y, nullptr, rstd, nullptr,
+                    x_row, gate_row, 0, rows * groups, H, groups, hg, eps};
+  const void* fn = dtype == PT_F32 ? pt::norm_fn<pt::Gated<float>::Fwd>(f)
+                                   : pt::norm_fn<pt::Gated<__bf16>::Fwd>(f);
+  void* args[] = {&a};
+  const int threads = pt::norm_threads(f.tpr);
+  return pt::ssm_launch(fn, pt::ssm_ceil(a.rows, threads / f.tpr), threads, stream, args);
+}
+
+int pt_gated_norm_bwd_workspace_bytes(int dtype, long long rows, int H, int groups, size_t* bytes) {
+  if (!bytes) return PT_ERR_NULL;
+  const int st = pt::check_gated(dtype, rows, H, groups);
+  if (st == PT_OK) *bytes = rows ? (size_t)pt::gated_parts(rows, H, groups) * H * 4 : 0;
+  return st;
+}
+
+int pt_gated_norm_bwd(int dtype, const void* x, long long x_row, const void* gate,
+                      long long gate_row, const float* w, const float* rstd, const void* gy,
+                      void* gx, void* ggate, float* gw, void* workspace, size_t workspace_bytes,
+                      long long rows, int H, int groups, void* stream) {
+  size_t need = 0;
+  int st = pt_gated_norm_bwd_workspace_bytes(dtype, rows, H, groups, &need);
+  if (st != PT_OK) return st;
+  if (!gw) return PT_ERR_NULL;
+  float* part = static_cast<float*>(workspace);
+  if (rows == 0) return pt::sum_columns(part, gw, 0, H, stream);
+  if (!x || !gate || !w || !rstd || !gy || !gx || !ggate) return PT_ERR_NULL;
+  if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
+  const int hg = H / groups;
+  const void* ptrs[] = {x, gate, w, gy, gx, ggate, workspace};
+  const pt::NormForm f = pt::norm_form(
+      hg, hg % 8 == 0 && x_row % 8 == 0 && gate_row % 8 == 0 && pt::all16(ptrs, 7));
+  pt::NormGradArgs g = {{x, gate, nullptr, w, nullptr, nullptr, nullptr, nullptr,
+                         const_cast<float*>(rstd), nullptr, x_row, gate_row, 0, rows * groups, H,
+                         groups, hg, 0.0f},
+                        gy, nullptr, gx, ggate, nullptr, part};
+  const void* fn = dtype == PT_F32 ? pt::norm_fn<pt::Gated<float>::Bwd>(f)
+                                   : pt::norm_fn<pt::Gated<__bf16>::Bwd>(f);
+  void* args[] = {&g};
+  st = pt::ssm_launch(fn, pt::norm_grid(g.f.rows, f, groups), pt::norm_threads(f.tpr), stream, args);
+  if (st != PT_OK) return st;
+  return pt::sum_columns(part, gw, pt::gated_parts(rows, H, groups), H, stream);
+}
+
+int pt_residual_norm_fwd(int dtype, int res_dtype, const void* x, long long x_row,
+                         const void* residual, long long res_row, const float* post_w,
+                         const float* scale, const float* w, void* y, void* sum, float* rstd,
+                         float* rstd_x, long long rows, int H, float eps, void* stream) {
+  const int st = pt::check_residual(dtype, res_dtype, rows, H);
+  if (st != PT_OK) return st;
+  if (rows == 0) return PT_OK;
+  if (!x || !w || !y || !sum) return PT_ERR_NULL;
+  const void* ptrs[] = {x, residual, post_w, scale, w, y, sum};
+  const pt::NormForm f = pt::norm_form(
+      H, H % 8 == 0 && x_row % 8 == 0 && res_row % 8 == 0 && pt::all16(ptrs, 7));
+  pt::NormArgs a = {x, nullptr, residual, w, post_w, scale, y, sum, rstd, rstd_x,
+                    x_row, 0, res_row, rows, H, 1, H, eps};
+  const void* fn = dtype == PT_F32 ? pt::norm_fn<pt::Residual<float, float>::Fwd>(f)
+                   : res_dtype == PT_F32 ? pt::norm_fn<pt::Residual<__bf16, float>::Fwd>(f)
+                                         : pt::norm_fn<pt::Residual<__bf16, __bf16>::Fwd>(f);
+  void* args[] = {&a};
+  const int threads = pt::norm_threads(f.tpr);
+  return pt::ssm_launch(fn, pt::ssm_ceil(rows, threads / f.tpr), threads, stream, args);
+}
+
+int pt_residual_norm_bwd_workspace_bytes(int dtype, long long rows, int H, int sums, size_t* bytes) {
+  if (!bytes) return PT_ERR_NULL;
+  const int st = pt::check_residual(dtype, dtype, rows, H);
+  if (st != PT_OK) return st;
+  if (sums < 1 || sums > 3) return PT_ERR_CONFIG;
+  *bytes = rows ? (size_t)pt::residual_parts(rows, H) * H * sums * 4 : 0;
+  return PT_OK;
+}
+
+int pt_residual_norm_bwd(int dtype, int res_dtype, const void* x, long long x_row,
+                         const void* residual, long long res_row, const float* post_w,
+                         const float* scale, const float* w, const float* rstd, const float* rstd_x,
+                         const void* gy, const void* gsum, void* gx, void* gresidual,
+                         float* gparams, void* workspace, size_t workspace_bytes, long long rows,
+                         int H, void* stream) {
+  const int sums = 1 + (scale != nullptr) + (post_w != nullptr);
+  size_t need = 0;
+  int st = pt::check_residual(dtype, res_dtype, rows, H);
+  if (st == PT_OK) st = pt_residual_norm_bwd_workspace_bytes(dtype, rows, H, sums, &need);
+  if (st != PT_OK) return st;
+  if (!gparams) return PT_ERR_NULL;
+  float* part = static_cast<float*>(workspace);
+  if (rows == 0) return pt::sum_columns(part, gparams, 0, sums * H, stream);
+  if (!x || !w || !rstd || (post_w && !rstd_x) || !gy || !gx) return PT_ERR_NULL;
+  if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
+  const void* ptrs[] = {x, residual, post_w, scale, w, gy, gsum, gx, gresidual, workspace};
+  const pt::NormForm f = pt::norm_form(
+      H, H % 8 == 0 && x_row % 8 == 0 && res_row % 8 == 0 && pt::all16(ptrs, 10));
+  pt::NormGradArgs g = {{x, nullptr, residual, w, post_w, scale, nullptr, nullptr,
+                         const_cast<float*>(rstd), const_cast<float*>(rstd_x), x_row, 0, res_row,
+                         rows, H, 1, H, 0.0f},
+                        gy, gsum, gx, nullptr, gresidual, part};
+  const void* fn = dtype == PT_F32 ? pt::norm_fn<pt::Residual<float, float>::Bwd>(f)
+                   : res_dtype == PT_F32 ? pt::norm_fn<pt::Residual<__bf16, float>::Bwd>(f)
+                                         : pt::norm_fn<pt::Residual<__bf16, __bf16>::Bwd>(f);
+  void* args[] = {&g};
+  st = pt::ssm_launch(fn, pt::norm_grid(rows, f, 1), pt::norm_threads(f.tpr), stream, args);
+  if (st != PT_OK) return st;
+  return pt::sum_columns(part, gparams, pt::residual_parts(rows, H), sums * H, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,322 @@
+// ssm_norm.hpp — the norms around a selective state space block, for MI355X
+// (gfx950, wave64).
+//
+// gated:    u = x silu(z), n = u rsqrt(mean over a group of u^2 + eps), y = n w
+// residual: f = x, or x rsqrt(mean x^2 + eps) pw;  r = residual + scale f;
+//           y = r rsqrt(mean r^2 + eps) w;  r and y are both outputs
+//
+// Bound by HBM: a few FLOP for each element read and written. A row (gated: a
+// group of a row) is held by TPR lanes, E values each in registers, from one
+// read of its inputs to one write of its outputs; sums of squares go over the
+// lanes and, from two waves on, through LDS. The backward passes walk rows
+// with a fixed grid, so that the weights' gradients add up in registers; the
+// workgroups' parts are added in a fixed order.
+
+#pragma once
+
+#include "ssm_common.hpp"
+
+namespace pt {
+
+constexpr int kNormMaxH = 16384;
+// Lanes of a workgroup whose rows take TPR lanes each.
+constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+
+struct NormArgs {
+  const void *x, *z;        // [rows, H]; z: the gate
+  const void* residual;     // [rows, H] or null
+  const float *w, *pw, *scale;  // [H]; pw and scale may be null
+  void *y, *r;              // [rows, H] contiguous
+  float *rstd, *rstd_x;     // saved for the backward: [rows groups], [rows] (or null)
+  long long x_row, z_row, res_row;
+  long long rows;           // gated: rows x groups
+  int H, groups, hg;        // hg = H / groups (residual: H)
+  float eps;
+};
+
+// E values of a row for lane `l` of TPR: eight neighbours each, or single ones.
+template <int E, int TPR, bool VEC>
+__device__ __forceinline__ int norm_col(int l, int i) {
+  return VEC ? (i / 8 * TPR + l) * 8 + i % 8 : i * TPR + l;
+}
+template <int E, int TPR, bool VEC, typename T>
+__device__ __forceinline__ void norm_load(const T* p, int l, int n, float (&v)[E]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+      float q[8] = {};
+      const int c = norm_col<E, TPR, VEC>(l, i);
+      if (c < n) load_vec<8>(p + c, q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i + j] = q[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = norm_col<E, TPR, VEC>(l, i);
+      v[i] = c < n ? load1(p + c) : 0.0f;
+    }
+  }
+}
+template <int E, int TPR, bool VEC, typename T>
+__device__ __forceinline__ void norm_store(T* p, int l, int n, const float (&v)[E]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+      float q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = v[i + j];
+      const int c = norm_col<E, TPR, VEC>(l, i);
+      if (c < n) store_vec<8>(p + c, q);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = norm_col<E, TPR, VEC>(l, i);
+      if (c < n) store1(p + c, v[i]);
+    }
+  }
+}
+
+// Sum over the TPR lanes of a row, in every one of them. Two buffers in turn,
+// so that one barrier a sum is enough.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float (*lds)[norm_threads(TPR) / 64], int& turn) {
+#pragma unroll
+  for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) v += lds[turn][k];
+    turn ^= 1;
+  }
+  return v;
+}
+
+template <typename T, int E, int TPR, bool VEC>
+__global__ __launch_bounds__(norm_threads(TPR)) void gated_fwd_kernel(NormArgs a) {
+  __shared__ float lds[2][norm_threads(TPR) / 64];
+  int turn = 0;
+  const int l = threadIdx.x % TPR;
+  const long long id = (long long)blockIdx.x * (norm_threads(TPR) / TPR) + threadIdx.x / TPR;
+  if (id >= a.rows) return;  // a row's lanes together
+  const long long row = id / a.groups;
+  const int c0 = (int)(id - row * a.groups) * a.hg;
+  float x[E], z[E], w[E], sum = 0.0f;
+  norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row + c0, l, a.hg, x);
+  norm_load<E, TPR, VEC>(static_cast<const T*>(a.z) + row * a.z_row + c0, l, a.hg, z);
+  norm_load<E, TPR, VEC>(a.w + c0, l, a.hg, w);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    x[i] *= z[i] * sigmoid_f32(z[i]);
+    sum = fmaf(x[i], x[i], sum);
+  }
+  sum = row_sum<TPR>(sum, lds, turn);
+  const float r = 1.0f / sqrtf(sum / (float)a.hg + a.eps);
+  if (a.rstd && l == 0) a.rstd[id] = r;
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[i];
+  norm_store<E, TPR, VEC>(static_cast<T*>(a.y) + row * a.H + c0, l, a.hg, x);
+}
+
+template <typename T, typename RT, int E, int TPR, bool VEC>
+__global__ __launch_bounds__(norm_threads(TPR)) void residual_fwd_kernel(NormArgs a) {
+  __shared__ float lds[2][norm_threads(TPR) / 64];
+  int turn = 0;
+  const int l = threadIdx.x % TPR;
+  const long long row = (long long)blockIdx.x * (norm_threads(TPR) / TPR) + threadIdx.x / TPR;
+  if (row >= a.rows) return;
+  float x[E], v[E];
+  norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row, l, a.H, x);
+  if (a.residual)
+    norm_load<E, TPR, VEC>(static_cast<const RT*>(a.residual) + row * a.res_row, l, a.H, v);
+  else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = 0.0f;
+  }
+  if (a.pw) {
+    float w[E], sum = 0.0f;
+    norm_load<E, TPR, VEC>(a.pw, l, a.H, w);
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum = fmaf(x[i], x[i], sum);
+    sum = row_sum<TPR>(sum, lds, turn);
+    const float r = 1.0f / sqrtf(sum / (float)a.H + a.eps);
+    if (a.rstd_x && l == 0) a.rstd_x[row] = r;
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[i];
+  }
+  float sum = 0.0f;
+  if (a.scale) {
+    float s[E];
+    norm_load<E, TPR, VEC>(a.scale, l, a.H, s);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = fmaf(s[i], x[i], v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] += x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) sum = fmaf(v[i], v[i], sum);
+  norm_store<E, TPR, VEC>(static_cast<RT*>(a.r) + row * a.H, l, a.H, v);
+  sum = row_sum<TPR>(sum, lds, turn);
+  const float r = 1.0f / sqrtf(sum / (float)a.H + a.eps);
+  if (a.rstd && l == 0) a.rstd[row] = r;
+  norm_load<E, TPR, VEC>(a.w, l, a.H, x);
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = v[i] * r * x[i];
+  norm_store<E, TPR, VEC>(static_cast<T*>(a.y) + row * a.H, l, a.H, v);
+}
+
+struct NormGradArgs {
+  NormArgs f;          // y and r unused
+  const void *gy, *gr; // [rows, H] contiguous; gr (residual) may be null
+  void *gx, *gz, *gres;  // [rows, H] contiguous; gres may be null
+  float* part;         // [grid][nparts][H]
+};
+
+// With n = u r, m = gy w:  gu = r (m - n mean(m n)).
+template <typename T, int E, int TPR, bool VEC>
+__global__ __launch_bounds__(norm_threads(TPR)) void gated_bwd_kernel(NormGradArgs g) {
+  __shared__ float lds[2][norm_threads(TPR) / 64];
+  const NormArgs& a = g.f;
+  int turn = 0;
+  const int l = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  constexpr int kRows = norm_threads(TPR) / TPR;
+  // A lane's rows are of one group: the grid is a multiple of the groups.
+  const long long first = (long long)blockIdx.x * kRows + sub;
+  const long long step = (long long)gridDim.x * kRows;
+  const int grp = (int)(first % a.groups), c0 = grp * a.hg;
+  float w[E], gw[E] = {};
+  norm_load<E, TPR, VEC>(a.w + c0, l, a.hg, w);
+  for (long long id = first; id < a.rows; id += step) {
+    const long long row = id / a.groups;
+    float x[E], z[E], gy[E], sum = 0.0f;
+    norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row + c0, l, a.hg, x);
+    norm_load<E, TPR, VEC>(static_cast<const T*>(a.z) + row * a.z_row + c0, l, a.hg, z);
+    norm_load<E, TPR, VEC>(static_cast<const T*>(g.gy) + row * a.H + c0, l, a.hg, gy);
+    const float r = a.rstd[id];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float n = x[i] * (z[i] * sigmoid_f32(z[i])) * r;
+      gw[i] = fmaf(gy[i], n, gw[i]);
+      gy[i] *= w[i];
+      sum = fmaf(gy[i], n, sum);
+    }
+    sum = row_sum<TPR>(sum, lds, turn) / (float)a.hg;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float sig = sigmoid_f32(z[i]), gate = z[i] * sig;
+      const float gu = r * (gy[i] - x[i] * gate * r * sum);
+      gy[i] = gu * gate;
+      z[i] = gu * x[i] * silu_grad_f32(z[i], sig);
+    }
+    norm_store<E, TPR, VEC>(static_cast<T*>(g.gx) + row * a.H + c0, l, a.hg, gy);
+    norm_store<E, TPR, VEC>(static_cast<T*>(g.gz) + row * a.H + c0, l, a.hg, z);
+  }
+  // One part a row of lanes: [grid kRows / groups][H].
+  norm_store<E, TPR, VEC>(g.part + first / a.groups * a.H + c0, l, a.hg, gw);
+}
+
+// With the sum r computed again from x and the residual, in FP32 whatever its
+// type: gr' = gr + rr (gy w - m mean(gy w m)), m = r rr; gf = scale gr';
+// gx = gf, or with n = x rx: rx (gf pw - n mean(gf pw n)).
+template <typename T, typename RT, int E, int TPR, bool VEC>
+__global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGradArgs g) {
+  __shared__ float lds[2][norm_threads(TPR) / 64];
+  const NormArgs& a = g.f;
+  int turn = 0;
+  const int l = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  constexpr int kRows = norm_threads(TPR) / TPR;
+  const long long first = (long long)blockIdx.x * kRows + sub;
+  const long long step = (long long)gridDim.x * kRows;
+  float gw[E] = {}, gs[E] = {}, gp[E] = {};
+  for (long long row = first; row < a.rows; row += step) {
+    float n[E], v[E], gy[E], w[E], sum = 0.0f, rx = 1.0f;
+    norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row, l, a.H, n);
+    norm_load<E, TPR, VEC>(static_cast<const T*>(g.gy) + row * a.H, l, a.H, gy);
+    if (a.residual)
+      norm_load<E, TPR, VEC>(static_cast<const RT*>(a.residual) + row * a.res_row, l, a.H, v);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = 0.0f;
+    }
+    const float rr = a.rstd[row];
+    float f[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = n[i];
+    if (a.pw) {
+      rx = a.rstd_x[row];
+      norm_load<E, TPR, VEC>(a.pw, l, a.H, w);
+#pragma unroll
+      for (int i = 0; i < E; ++i) n[i] *= rx, f[i] = n[i] * w[i];
+    }
+    if (a.scale) {
+      norm_load<E, TPR, VEC>(a.scale, l, a.H, w);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = fmaf(w[i], f[i], v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] += f[i];
+    }
+    norm_load<E, TPR, VEC>(a.w, l, a.H, w);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      v[i] *= rr;
+      gw[i] = fmaf(gy[i], v[i], gw[i]);
+      gy[i] *= w[i];
+      sum = fmaf(gy[i], v[i], sum);
+    }
+    sum = row_sum<TPR>(sum, lds, turn) / (float)a.H;
+#pragma unroll
+    for (int i = 0; i < E; ++i) gy[i] = rr * (gy[i] - v[i] * sum);
+    if (g.gr) {
+      norm_load<E, TPR, VEC>(static_cast<const RT*>(g.gr) + row * a.H, l, a.H, v);
+#pragma unroll
+      for (int i = 0; i < E; ++i) gy[i] += v[i];
+    }
+    if (g.gres) norm_store<E, TPR, VEC>(static_cast<RT*>(g.gres) + row * a.H, l, a.H, gy);
+    if (a.scale) {
+      norm_load<E, TPR, VEC>(a.scale, l, a.H, w);
+#pragma unroll
+      for (int i = 0; i < E; ++i) gs[i] = fmaf(gy[i], f[i], gs[i]), gy[i] *= w[i];
+    }
+    if (a.pw) {
+      norm_load<E, TPR, VEC>(a.pw, l, a.H, w);
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        gp[i] = fmaf(gy[i], n[i], gp[i]);
+        gy[i] *= w[i];
+        sum = fmaf(gy[i], n[i], sum);
+      }
+      sum = row_sum<TPR>(sum, lds, turn) / (float)a.H;
+#pragma unroll
+      for (int i = 0; i < E; ++i) gy[i] = rx * (gy[i] - n[i] * sum);
+    }
+    norm_store<E, TPR, VEC>(static_cast<T*>(g.gx) + row * a.H, l, a.H, gy);
+  }
+  const int np = 1 + (a.scale != nullptr) + (a.pw != nullptr);
+  float* part = g.part + first * np * a.H;
+  norm_store<E, TPR, VEC>(part, l, a.H, gw);
+  if (a.scale) norm_store<E, TPR, VEC>(part + a.H, l, a.H, gs);
+  if (a.pw) norm_store<E, TPR, VEC>(part + (long long)(np - 1) * a.H, l, a.H, gp);
+}
+
+// out[c] = sum over k of part[k][c], 64 columns by 4 ranges a workgroup.
+__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part,
+                                                         float* __restrict__ out, long long parts,
+                                                         int cols) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = (int)blockIdx.x * 64 + lane;
+  float v = 0.0f;
+  if (c < cols)
+    for (long long k = w; k < parts; k += 4) v += part[k * cols + c];
+  sums[w][lane] = v;
+  __syncthreads();
+  if (w == 0 && c < cols) out[c] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+}
+
+}  // namespace pt

@@ -1,0 +1,547 @@
+"""Operators of a selective state space block on MI355X, channels last.
+
+Where S4ConvD (``pathtile_amd.s4convd``) runs a diagonal state space as one
+convolution, whose kernel is the same at every token, the selective form takes
+the step size and the in- and output maps from the tokens themselves. That is
+no convolution any more: it is a scan over the sequence, of any length, with a
+state that a server carries from token to token. The operators, each for
+training (gradients of every input), for prompts and for single tokens:
+
+* ``causal_conv``, ``causal_conv_step``       short causal depthwise convolution
+* ``selective_scan``, ``selective_scan_step`` the scan
+* ``gated_norm``     RMS norm of ``x * silu(gate)``, after the scan
+* ``residual_norm``  post-norm, scale, residual and the next block's pre-norm
+
+Activations are float32 or bfloat16, one type in a call; weights, scan states
+and their gradients are float32. Arithmetic is FP32 and every output is rounded
+once. Inputs may be views whose channels are contiguous (a slice of a
+projection's output); outputs are contiguous. Launches go on torch's current
+stream of the tensors' device. Gradients are first order and deterministic.
+Nothing falls back to PyTorch: without the native library every call raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .runtime import _call, _ptr
+
+MAX_TAPS = 8
+MAX_STATES = 64
+MAX_NORM_CHANNELS = 16384
+_TYPES = {torch.float32: _lib.PT_F32, torch.bfloat16: _lib.PT_BF16}
+
+
+# --- argument checks -----------------------------------------------------------
+def _activation(x: torch.Tensor, ndim: int, what: str) -> int:
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    if x.dtype not in _TYPES:
+        raise ValueError("x must be float32 or bfloat16")
+    if x.ndim != ndim:
+        raise ValueError(f"Expected x{what}")
+    return _TYPES[x.dtype]
+
+
+def _like(t: torch.Tensor, x: torch.Tensor, shape: tuple, name: str) -> None:
+    """`t` has x's type and device and the given shape."""
+    if t.dtype != x.dtype or t.device != x.device or t.shape != shape:
+        raise ValueError(f"{name} must be a {str(x.dtype)[6:]} tensor of shape {tuple(shape)} "
+                         "on x's device")
+
+
+def _weights(t: torch.Tensor | None, x: torch.Tensor, shape: tuple, name: str):
+    """A float32 parameter of that shape, contiguous; None stays None."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != x.device or t.shape != shape:
+        raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)} on x's device")
+    return t.contiguous()
+
+
+def _lengths(t: torch.Tensor | None, x: torch.Tensor):
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or t.device != x.device or t.shape != x.shape[:1]:
+        raise ValueError(f"lengths must be an int32 tensor of shape {(x.shape[0],)} on x's device")
+    # int64 lengths are clamped before they lose their upper half
+    return (t if t.dtype == torch.int32 else t.clamp(0, x.shape[1]).int()).contiguous()
+
+
+def _slots(t: torch.Tensor | None, x: torch.Tensor, pool: int):
+    if t is None:
+        if pool < x.shape[0]:
+            raise ValueError(f"{x.shape[0]} sequences need as many states, got {pool}")
+        return None
+    if t.dtype != torch.int32 or t.device != x.device or t.shape != x.shape[:1]:
+        raise ValueError(f"slots must be an int32 tensor of shape {(x.shape[0],)} on x's device")
+    return t.contiguous()
+
+
+def _pool(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, row: tuple) -> int:
+    if (t.dtype != dtype or t.device != x.device or t.ndim != 3 or t.shape[1:] != row
+            or not t.is_contiguous()):
+        raise ValueError(f"state must be a contiguous {str(dtype)[6:]} tensor of shape "
+                         f"{('pool', *row)} on x's device")
+    return t.shape[0]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` with its last dimension contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor, n: int) -> list[int]:
+    """The first n strides in elements; 0 along a dimension of one."""
+    return [s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape)]
+
+
+def _opt(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _asks_gradient(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _bytes(query: str, *args: Any) -> int:
+    out = ctypes.c_size_t(0)
+    _lib.check(getattr(_lib.load(), query)(*args, ctypes.byref(out)), query)
+    return int(out.value)
+
+
+def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+
+
+def _form(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+def _save(ctx: Any, *tensors: torch.Tensor | None) -> None:
+    ctx.forms = [_form(t) for t in tensors]
+    ctx.save_for_backward(*tensors)
+
+
+def _saved(ctx: Any) -> list:
+    """The saved tensors, which a hook may have given back in other strides
+    but not in another shape, type or place."""
+    got = ctx.saved_tensors
+    for t, form in zip(got, ctx.forms):
+        if _form(t) != form:
+            raise RuntimeError(f"saved tensor {form} was unpacked as {_form(t)}")
+    return list(got)
+
+
+# --- the short causal convolution ------------------------------------------------
+def _conv_forward(x, weight, bias, state, lengths, silu, return_state):
+    B, L, H = x.shape
+    K = weight.shape[1]
+    y = torch.empty(B, L, H, dtype=x.dtype, device=x.device)
+    out = torch.empty(B, K - 1, H, dtype=x.dtype, device=x.device) if return_state else None
+    _call(_lib.load().pt_causal_conv_fwd, x.device, _TYPES[x.dtype], _ptr(x), *_strides(x, 2),
+          _ptr(weight), _opt(bias), _opt(state), _opt(lengths), _ptr(y), _opt(out),
+          B, L, H, K, silu)
+    return y, out
+
+
+class CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, weight, bias, state, lengths, silu: bool, return_state: bool):
+        y, out = _conv_forward(x, weight, bias, state, lengths, silu, return_state)
+        _save(ctx, x, weight, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return (y, out) if return_state else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gy, gout=None):
+        x, weight, bias, state, lengths = _saved(ctx)
+        x, weight = _rows(x), weight.contiguous()
+        bias, state, lengths = (t if t is None else t.contiguous() for t in (bias, state, lengths))
+        B, L, H = x.shape
+        K = weight.shape[1]
+        gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else gy.contiguous()
+        gout = None if gout is None else gout.contiguous()
+        gx, gw = torch.empty_like(gy), torch.empty_like(weight)
+        gb = None if bias is None else torch.empty_like(bias)
+        gs = torch.empty_like(state) if ctx.needs_input_grad[3] else None
+        kind = _TYPES[x.dtype]
+        ws = _workspace(_bytes("pt_causal_conv_bwd_workspace_bytes", kind, B, L, H, K), x)
+        _call(_lib.load().pt_causal_conv_bwd, x.device, kind, _ptr(x), *_strides(x, 2),
+              _ptr(weight), _opt(bias), _opt(state), _opt(lengths), _ptr(gy), _opt(gout), _ptr(gx),
+              _ptr(gw), _opt(gb), _opt(gs), _opt(ws), 0 if ws is None else ws.numel(),
+              B, L, H, K, ctx.silu)
+        return gx, gw, gb, gs, None, None, None
+
+
+def _check_taps(weight: torch.Tensor, H: int, x: torch.Tensor):
+    if weight.ndim != 2 or not 1 <= weight.shape[1] <= MAX_TAPS:
+        raise ValueError(f"Expected weight[H,K] with 1<=K<={MAX_TAPS}")
+    return _weights(weight, x, (H, weight.shape[1]), "weight")
+
+
+def _activation_name(activation: str | None) -> bool:
+    if activation not in ("silu", None):
+        raise ValueError("activation must be 'silu' or None")
+    return activation == "silu"
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                activation: str | None = "silu", state: torch.Tensor | None = None,
+                lengths: torch.Tensor | None = None, return_state: bool = False):
+    """``y[b,t,h] = act(bias[h] + sum_j weight[h,j] x[b,t-(K-1)+j,h])``.
+
+    ``x`` [B, L, H]; ``weight`` [H, K], K <= 8; ``state`` [B, K-1, H] in x's
+    type holds the tokens before the first (default: zeros); ``lengths`` [B]
+    (default: L) counts each sequence's tokens: past them y is 0. With
+    ``return_state`` the result is ``(y, state)``, the sequence's last K - 1
+    tokens, with which a later call or ``causal_conv_step`` goes on."""
+    _activation(x, 3, "[B,L,H]")
+    B, L, H = x.shape
+    silu = _activation_name(activation)
+    weight, bias = _check_taps(weight, H, x), _weights(bias, x, (H,), "bias")
+    K = weight.shape[1]
+    if state is not None:
+        _like(state, x, (B, K - 1, H), "state")
+        state = state.contiguous()
+    lengths = _lengths(lengths, x)
+    if x.numel() == 0:  # no tokens: the state as it was
+        y = x.new_empty(x.shape) + 0 * (weight.sum() + (0 if bias is None else bias.sum())).to(x.dtype)
+        last = x.new_zeros(B, K - 1, H) if state is None else state.clone()
+        return (y, last) if return_state else y
+    x = _rows(x)
+    if _asks_gradient(x, weight, bias, state):
+        return CausalConv.apply(x, weight, bias, state, lengths, silu, return_state)
+    y, out = _conv_forward(x, weight, bias, state, lengths, silu, return_state)
+    return (y, out) if return_state else y
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
+                     bias: torch.Tensor | None = None, *, activation: str | None = "silu",
+                     slots: torch.Tensor | None = None) -> torch.Tensor:
+    """One token ``x`` [B, H] of each of B sequences: y [B, H], no gradient.
+
+    ``state`` [pool, K-1, H] (x's type) is updated in place at rows
+    ``slots[b]`` (int32, different from each other; default: row b). A slot
+    outside the pool marks a row without a sequence: its y is 0."""
+    kind = _activation(x, 2, "[B,H]")
+    B, H = x.shape
+    silu = _activation_name(activation)
+    weight, bias = _check_taps(weight, H, x), _weights(bias, x, (H,), "bias")
+    K = weight.shape[1]
+    pool = _pool(state, x, x.dtype, (K - 1, H))
+    slots = _slots(slots, x, pool)
+    x = _rows(x)
+    y = torch.empty(B, H, dtype=x.dtype, device=x.device)
+    if y.numel():
+        _call(_lib.load().pt_causal_conv_step, x.device, kind, _ptr(x), *_strides(x, 1),
+              _ptr(weight), _opt(bias), _ptr(state), _opt(slots), _ptr(y), B, H, K, pool, silu)
+    return y
+
+
+# --- the scan ------------------------------------------------------------------
+def _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus):
+    """pt_scan_inputs for x, dt [B, L, H] and b, c [B, L, G, N], or without L."""
+    H, (G, N) = x.shape[-1], b.shape[-2:]
+    L = x.shape[1] if x.ndim == 3 else 1
+    n = x.ndim - 1
+    xs, ds, bs, cs = _strides(x, n), _strides(dt, n), _strides(b, n + 1), _strides(c, n + 1)
+    if n == 1:
+        xs, ds, bs, cs = ([s[0], 0, *s[1:]] for s in (xs, ds, bs, cs))
+    return _lib.ScanInputs(_ptr(x), _ptr(dt), _ptr(b), _ptr(c), _ptr(A), _opt(D), _opt(dt_bias),
+                           _opt(state), _opt(lengths), *xs, *ds, *bs, *cs, _TYPES[x.dtype],
+                           x.shape[0], L, H, N, G, softplus)
+
+
+def _scan_sizes(inputs) -> tuple[int, int, int]:
+    out = [ctypes.c_size_t(0) for _ in range(3)]
+    _lib.check(_lib.load().pt_selective_scan_sizes(ctypes.byref(inputs), *map(ctypes.byref, out)),
+               "pt_selective_scan_sizes")
+    return tuple(int(v.value) for v in out)
+
+
+def _scan_forward(x, dt, A, b, c, D, dt_bias, state, lengths, softplus, return_state, train):
+    B, L, H = x.shape
+    N = b.shape[-1]
+    inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus)
+    ws_bytes, saved_bytes, _ = _scan_sizes(inputs)
+    y = torch.empty(B, L, H, dtype=x.dtype, device=x.device)
+    out = torch.empty(B, H, N, dtype=torch.float32, device=x.device) if return_state else None
+    saved = (torch.empty(saved_bytes // 4, dtype=torch.float32, device=x.device)
+             if train else None)
+    ws = _workspace(ws_bytes, x)
+    _call(_lib.load().pt_selective_scan_fwd, x.device, ctypes.byref(inputs), _ptr(y), _opt(out),
+          _opt(saved), _opt(ws), ws_bytes)
+    return y, out, saved
+
+
+class SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, dt, A, b, c, D, dt_bias, state, lengths, softplus: bool,
+                return_state: bool):
+        y, out, saved = _scan_forward(x, dt, A, b, c, D, dt_bias, state, lengths, softplus,
+                                      return_state, True)
+        _save(ctx, x, dt, A, b, c, D, dt_bias, state, lengths, saved)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return (y, out) if return_state else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gy, gout=None):
+        x, dt, A, b, c, D, dt_bias, state, lengths, saved = _saved(ctx)
+        x, dt = _rows(x), _rows(dt)
+        b, c = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (b, c))
+        A, D, dt_bias, state, lengths, saved = (
+            t if t is None else t.contiguous() for t in (A, D, dt_bias, state, lengths, saved))
+        gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else gy.contiguous()
+        gout = None if gout is None else gout.contiguous()
+        inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, ctx.softplus)
+        ws = _workspace(_scan_sizes(inputs)[2], x)
+        gx, gdt, ga = torch.empty_like(gy), torch.empty_like(gy), torch.empty_like(A)
+        gb, gc = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (b, c))
+        gd, gbias = (None if t is None else torch.empty_like(t) for t in (D, dt_bias))
+        gs = torch.empty_like(state) if ctx.needs_input_grad[7] else None
+        _call(_lib.load().pt_selective_scan_bwd, x.device, ctypes.byref(inputs), _ptr(gy),
+              _ptr(saved), _opt(gout), _ptr(gx), _ptr(gdt), _ptr(ga), _ptr(gb), _ptr(gc), _opt(gd),
+              _opt(gbias), _opt(gs), _opt(ws), 0 if ws is None else ws.numel())
+        return gx, gdt, ga, gb, gc, gd, gbias, gs, None, None, None
+
+
+def _check_scan(x, dt, A, B, C, D, dt_bias):
+    """The scan's inputs as the kernels take them; B and C as [..., G, N]."""
+    H = x.shape[-1]
+    _like(dt, x, x.shape, "dt")
+    if A.ndim != 2 or not 1 <= A.shape[1] <= MAX_STATES:
+        raise ValueError(f"Expected A[H,N] with 1<=N<={MAX_STATES}")
+    N = A.shape[1]
+    A = _weights(A, x, (H, N), "A")
+    D, dt_bias = _weights(D, x, (H,), "D"), _weights(dt_bias, x, (H,), "dt_bias")
+    if B.ndim == x.ndim:
+        B = B.unsqueeze(-2)
+    if C.ndim == x.ndim:
+        C = C.unsqueeze(-2)
+    if B.ndim != x.ndim + 1 or B.shape[-2] < 1 or H % B.shape[-2]:
+        raise ValueError("Expected B and C [..., N] or [..., G, N] with H divisible by G")
+    shape = (*x.shape[:-1], B.shape[-2], N)
+    _like(B, x, shape, "B")
+    _like(C, x, shape, "C")
+    return _rows(x), _rows(dt), A, _rows(B), _rows(C), D, dt_bias
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                   C: torch.Tensor, D: torch.Tensor | None = None, *,
+                   dt_bias: torch.Tensor | None = None, softplus: bool = True,
+                   state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   return_state: bool = False):
+    """For each sequence b and channel h, over its tokens t, with
+    ``d = softplus(dt[b,t,h] + dt_bias[h])`` (or without softplus):
+
+    ``s[n] = exp(d A[h,n]) s[n] + d x[b,t,h] B[b,t,g,n]``
+    ``y[b,t,h] = sum_n C[b,t,g,n] s[n] + D[h] x[b,t,h]``
+
+    ``x``, ``dt`` [B, L, H]; ``A`` [H, N], N <= 64; ``B``, ``C`` [B, L, N], or
+    [B, L, G, N] where each of G groups of H / G neighbouring channels g has
+    its own. ``state`` [B, H, N] float32 is the first state (default: zeros),
+    ``lengths`` [B] (default: L) counts each sequence's tokens: past them y is
+    0 and the state stays. With ``return_state`` the result is ``(y, state)``.
+    For gradients the forward keeps the states before every 16 tokens (N / 4
+    bytes for each value of x)."""
+    _activation(x, 3, "[B,L,H]")
+    x, dt, A, B, C, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
+    if state is not None:
+        state = _weights(state, x, (x.shape[0], x.shape[2], A.shape[1]), "state")
+    lengths = _lengths(lengths, x)
+    if x.numel() == 0:
+        params = [t.sum() for t in (A, D, dt_bias) if t is not None]
+        y = x.new_empty(x.shape) + 0 * sum(params).to(x.dtype)
+        last = (x.new_zeros(x.shape[0], *A.shape, dtype=torch.float32) if state is None
+                else state.clone())
+        return (y, last) if return_state else y
+    if _asks_gradient(x, dt, A, B, C, D, dt_bias, state):
+        return SelectiveScan.apply(x, dt, A, B, C, D, dt_bias, state, lengths, bool(softplus),
+                                   return_state)
+    y, out, _ = _scan_forward(x, dt, A, B, C, D, dt_bias, state, lengths, bool(softplus),
+                              return_state, False)
+    return (y, out) if return_state else y
+
+
+def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                        C: torch.Tensor, state: torch.Tensor, D: torch.Tensor | None = None, *,
+                        dt_bias: torch.Tensor | None = None, softplus: bool = True,
+                        slots: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of each of B sequences: ``x``, ``dt`` [B, H], ``B``, ``C``
+    [B, N] or [B, G, N]; y [B, H], no gradient. ``state`` [pool, H, N] float32
+    is updated in place at rows ``slots[b]``, as in ``causal_conv_step``."""
+    _activation(x, 2, "[B,H]")
+    x, dt, A, B, C, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
+    pool = _pool(state, x, torch.float32, tuple(A.shape))
+    slots = _slots(slots, x, pool)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel():
+        inputs = _scan_inputs(x, dt, A, B, C, D, dt_bias, None, None, bool(softplus))
+        _call(_lib.load().pt_selective_scan_step, x.device, ctypes.byref(inputs), _ptr(state),
+              _opt(slots), pool, _ptr(y))
+    return y
+
+
+# --- the norms -----------------------------------------------------------------
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """[..., H] as [rows, H] with contiguous channels."""
+    return _rows(t if t.ndim == 2 else t.reshape(-1, t.shape[-1]))
+
+
+def _norm_input(x: torch.Tensor) -> int:
+    if x.ndim < 1:
+        raise ValueError("Expected x[...,H]")
+    kind = _activation(x, x.ndim, "")
+    if x.shape[-1] < 1:
+        raise ValueError("Expected x[...,H] with H>=1")
+    return kind
+
+
+def _gated_forward(x, gate, weight, eps, groups, train):
+    rows, H = x.shape
+    y = torch.empty(rows, H, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(rows * groups, dtype=torch.float32, device=x.device) if train else None
+    _call(_lib.load().pt_gated_norm_fwd, x.device, _TYPES[x.dtype], _ptr(x), *_strides(x, 1),
+          _ptr(gate), *_strides(gate, 1), _ptr(weight), _ptr(y), _opt(rstd), rows, H, groups, eps)
+    return y, rstd
+
+
+class GatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, gate, weight, eps: float, groups: int):
+        y, rstd = _gated_forward(x, gate, weight, eps, groups, True)
+        _save(ctx, x, gate, weight, rstd)
+        ctx.groups = groups
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gy):
+        x, gate, weight, rstd = _saved(ctx)
+        x, gate, weight, rstd = _rows(x), _rows(gate), weight.contiguous(), rstd.contiguous()
+        rows, H = x.shape
+        gy = gy.contiguous()
+        gx, gg, gw = torch.empty_like(gy), torch.empty_like(gy), torch.empty_like(weight)
+        kind = _TYPES[x.dtype]
+        ws = _workspace(_bytes("pt_gated_norm_bwd_workspace_bytes", kind, rows, H, ctx.groups), x)
+        _call(_lib.load().pt_gated_norm_bwd, x.device, kind, _ptr(x), *_strides(x, 1), _ptr(gate),
+              *_strides(gate, 1), _ptr(weight), _ptr(rstd), _ptr(gy), _ptr(gx), _ptr(gg), _ptr(gw),
+              _opt(ws), 0 if ws is None else ws.numel(), rows, H, ctx.groups)
+        return gx, gg, gw, None, None
+
+
+def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, *, groups: int = 1,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``u = x * silu(gate)``, ``y = u / sqrt(mean(u^2) + eps) * weight``, the
+    mean over each of ``groups`` equal parts of the channels. ``x`` and
+    ``gate`` [..., H], ``weight`` [H], up to 16384 channels a group."""
+    _norm_input(x)
+    H = x.shape[-1]
+    _like(gate, x, x.shape, "gate")
+    weight = _weights(weight, x, (H,), "weight")
+    if groups < 1 or H % groups or H // groups > MAX_NORM_CHANNELS:
+        raise ValueError(f"groups must divide H into parts of at most {MAX_NORM_CHANNELS} channels")
+    shape, x, gate = x.shape, _flat(x), _flat(gate)
+    if _asks_gradient(x, gate, weight):
+        return GatedNorm.apply(x, gate, weight, float(eps), int(groups)).view(shape)
+    return _gated_forward(x, gate, weight, float(eps), int(groups), False)[0].view(shape)
+
+
+def _residual_forward(x, residual, weight, post_weight, scale, eps, train):
+    rows, H = x.shape
+    kind = _TYPES[x.dtype]
+    res = x if residual is None else residual
+    y = torch.empty(rows, H, dtype=x.dtype, device=x.device)
+    out = torch.empty(rows, H, dtype=res.dtype, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if train else None
+    rstd_x = torch.empty_like(rstd) if train and post_weight is not None else None
+    _call(_lib.load().pt_residual_norm_fwd, x.device, kind, _TYPES[res.dtype], _ptr(x),
+          *_strides(x, 1), _opt(residual), *_strides(res, 1), _opt(post_weight), _opt(scale),
+          _ptr(weight), _ptr(y), _ptr(out), _opt(rstd), _opt(rstd_x), rows, H, eps)
+    return y, out, rstd, rstd_x
+
+
+class ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, residual, weight, post_weight, scale, eps: float):
+        y, out, rstd, rstd_x = _residual_forward(x, residual, weight, post_weight, scale, eps, True)
+        _save(ctx, x, residual, weight, post_weight, scale, rstd, rstd_x)
+        ctx.out_type = out.dtype
+        ctx.set_materialize_grads(False)
+        return y, out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gy, gout):
+        x, residual, weight, post_weight, scale, rstd, rstd_x = _saved(ctx)
+        x, residual = _rows(x), None if residual is None else _rows(residual)
+        weight, post_weight, scale, rstd, rstd_x = (
+            t if t is None else t.contiguous() for t in (weight, post_weight, scale, rstd, rstd_x))
+        rows, H = x.shape
+        gy = torch.zeros(rows, H, dtype=x.dtype, device=x.device) if gy is None else gy.contiguous()
+        gout = None if gout is None else gout.contiguous()
+        gx = torch.empty_like(gy)
+        gres = (torch.empty(rows, H, dtype=residual.dtype, device=x.device)
+                if ctx.needs_input_grad[1] else None)
+        sums = 1 + (scale is not None) + (post_weight is not None)
+        params = torch.empty(sums, H, dtype=torch.float32, device=x.device)
+        kind = _TYPES[x.dtype]
+        ws = _workspace(_bytes("pt_residual_norm_bwd_workspace_bytes", kind, rows, H, sums), x)
+        _call(_lib.load().pt_residual_norm_bwd, x.device, kind, _TYPES[ctx.out_type], _ptr(x),
+              *_strides(x, 1), _opt(residual), *_strides(x if residual is None else residual, 1),
+              _opt(post_weight), _opt(scale), _ptr(weight), _ptr(rstd), _opt(rstd_x), _ptr(gy),
+              _opt(gout), _ptr(gx), _opt(gres), _ptr(params), _opt(ws),
+              0 if ws is None else ws.numel(), rows, H)
+        gp = None if post_weight is None else params[-1]
+        gs = None if scale is None else params[1]
+        return gx, gres, params[0], gp, gs, None
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *,
+                  post_weight: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
+    """The end of one block and the start of the next: ``(y, sum)`` with
+
+    ``f = x``, or with ``post_weight``  ``x / sqrt(mean(x^2) + eps) * post_weight``
+    ``sum = residual + scale * f``,  ``y = sum / sqrt(mean(sum^2) + eps) * weight``
+
+    ``x`` [..., H] is the block's output; ``residual`` has its shape and its
+    type or float32, and gives ``sum`` its type (None: zeros in x's type);
+    ``weight``, ``post_weight`` and ``scale`` are [H], H <= 16384."""
+    _norm_input(x)
+    H = x.shape[-1]
+    if H > MAX_NORM_CHANNELS:
+        raise ValueError(f"residual_norm takes up to {MAX_NORM_CHANNELS} channels")
+    weight = _weights(weight, x, (H,), "weight")
+    post_weight = _weights(post_weight, x, (H,), "post_weight")
+    scale = _weights(scale, x, (H,), "scale")
+    shape = x.shape
+    if residual is not None:
+        if (residual.dtype not in (x.dtype, torch.float32) or residual.device != x.device
+                or residual.shape != shape):
+            raise ValueError(f"residual must be of shape {tuple(shape)}, in x's type or float32, "
+                             "on x's device")
+        residual = _flat(residual)
+    x = _flat(x)
+    if _asks_gradient(x, residual, weight, post_weight, scale):
+        y, out = ResidualNorm.apply(x, residual, weight, post_weight, scale, float(eps))
+    else:
+        y, out, _, _ = _residual_forward(x, residual, weight, post_weight, scale, float(eps), False)
+    return y.view(shape), out.view(shape)
+
+
+__all__ = [
+    "MAX_TAPS", "MAX_STATES", "MAX_NORM_CHANNELS",
+    "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step",
+    "gated_norm", "residual_norm",
+]

@@ -1,0 +1,167 @@
+"""A small language model of selective state space blocks, which runs the
+operators of ``pathtile_amd.selective`` together as they are meant to be used:
+training on whole sequences, prompts of different lengths (whole or in
+chunks), and single tokens from a pool of states.
+
+One block, with M model channels and H = ``expand`` M inner ones::
+
+    x, z     = split(in_proj(u))                    u: normed input [B, L, M]
+    x        = causal_conv(x)
+    dt, B, C = split(x_proj(x)); dt = dt_proj(dt)
+    y        = selective_scan(x, dt, A, B, C, D)
+    out      = out_proj(gated_norm(y, z))
+
+and ``residual_norm`` closes it: the block's output is normed, scaled and
+added to the residual stream, which is float32, and normed for the next block.
+Linear layers and activations are ``dtype``; the operators' weights float32::
+
+    model = SelectiveModel(vocab=256).cuda()
+    logits = model(tokens)                                  # training
+    cache = model.new_cache(pool=8)
+    logits = model.prompt(tokens, cache, slots, lengths)    # [B, vocab]
+    logits = model.step(next_tokens, cache, slots)          # [B, vocab]
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+from torch import nn
+
+from .selective import (
+    causal_conv, causal_conv_step, gated_norm, residual_norm, selective_scan, selective_scan_step,
+)
+
+
+@dataclass
+class SelectiveCache:
+    """The states of ``pool`` sequences: per block the convolution's last
+    tokens [pool, K-1, H] and the scan's states [pool, H, N]."""
+
+    conv: list[torch.Tensor]
+    scan: list[torch.Tensor]
+
+    def clear(self, slots: torch.Tensor) -> None:
+        """New sequences at ``slots``."""
+        for pool in (*self.conv, *self.scan):
+            pool[slots.long()] = 0
+
+
+class SelectiveBlock(nn.Module):
+    def __init__(self, hidden: int, state: int = 16, taps: int = 4, expand: int = 2,
+                 dt_rank: int | None = None, groups: int = 1,
+                 dtype: torch.dtype = torch.bfloat16) -> None:
+        super().__init__()
+        inner = expand * hidden
+        self.inner, self.state, self.taps, self.groups = inner, state, taps, groups
+        self.dt_rank = dt_rank or max(1, -(-hidden // 16))
+        self.in_proj = nn.Linear(hidden, 2 * inner, bias=False, dtype=dtype)
+        self.x_proj = nn.Linear(inner, self.dt_rank + 2 * groups * state, bias=False, dtype=dtype)
+        self.dt_proj = nn.Linear(self.dt_rank, inner, bias=False, dtype=dtype)
+        self.out_proj = nn.Linear(inner, hidden, bias=False, dtype=dtype)
+        self.conv_weight = nn.Parameter((2 * torch.rand(inner, taps) - 1) / math.sqrt(taps))
+        self.conv_bias = nn.Parameter(torch.zeros(inner))
+        # -A = 1 .. state, and steps between 1e-3 and 1e-1 at dt = 0
+        self.log_A = nn.Parameter(torch.arange(1, state + 1).float().log().repeat(inner, 1))
+        step = torch.exp(torch.rand(inner) * math.log(100.0) + math.log(1e-3))
+        self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
+        self.D = nn.Parameter(torch.ones(inner))
+        self.norm_weight = nn.Parameter(torch.ones(inner))
+
+    def _maps(self, x: torch.Tensor):
+        """dt, B and C of the convolved tokens."""
+        n = self.groups * self.state
+        dt, b, c = self.x_proj(x).split((self.dt_rank, n, n), -1)
+        return (self.dt_proj(dt), b.unflatten(-1, (self.groups, self.state)),
+                c.unflatten(-1, (self.groups, self.state)))
+
+    def forward(self, u: torch.Tensor, conv=None, scan=None, lengths=None,
+                return_state: bool = False):
+        """u [B, L, M] -> [B, L, M], with the new states where asked for."""
+        x, z = self.in_proj(u).chunk(2, -1)
+        x = causal_conv(x, self.conv_weight, self.conv_bias, state=conv, lengths=lengths,
+                        return_state=return_state)
+        x, conv = x if return_state else (x, None)
+        dt, b, c = self._maps(x)
+        y = selective_scan(x, dt, -self.log_A.exp(), b, c, self.D, dt_bias=self.dt_bias,
+                           state=scan, lengths=lengths, return_state=return_state)
+        y, scan = y if return_state else (y, None)
+        out = self.out_proj(gated_norm(y, z, self.norm_weight))
+        return (out, conv, scan) if return_state else out
+
+    def step(self, u: torch.Tensor, conv: torch.Tensor, scan: torch.Tensor, slots=None):
+        """u [B, M] -> [B, M]; the pools are updated in place."""
+        x, z = self.in_proj(u).chunk(2, -1)
+        x = causal_conv_step(x, self.conv_weight, conv, self.conv_bias, slots=slots)
+        dt, b, c = self._maps(x)
+        y = selective_scan_step(x, dt, -self.log_A.exp(), b, c, scan, self.D,
+                                dt_bias=self.dt_bias, slots=slots)
+        return self.out_proj(gated_norm(y, z, self.norm_weight))
+
+
+class SelectiveModel(nn.Module):
+    def __init__(self, vocab: int = 256, hidden: int = 128, blocks: int = 4, state: int = 16,
+                 taps: int = 4, expand: int = 2, groups: int = 1,
+                 dtype: torch.dtype = torch.bfloat16) -> None:
+        super().__init__()
+        self.dtype = dtype
+        self.embedding = nn.Embedding(vocab, hidden)
+        self.blocks = nn.ModuleList(
+            SelectiveBlock(hidden, state, taps, expand, groups=groups, dtype=dtype)
+            for _ in range(blocks))
+        # pre-norms of the blocks and of the head; post-norms and scales of the blocks
+        self.pre = nn.ParameterList(torch.ones(hidden) for _ in range(blocks + 1))
+        self.post = nn.ParameterList(torch.ones(hidden) for _ in range(blocks))
+        self.scale = nn.ParameterList(
+            torch.full((hidden,), blocks ** -0.5) for _ in range(blocks))
+        self.head = nn.Linear(hidden, vocab, bias=False, dtype=dtype)
+
+    def _run(self, tokens: torch.Tensor, block_out) -> torch.Tensor:
+        """The normed output of the last block; ``block_out(i, u)`` runs block i."""
+        r = self.embedding(tokens)
+        u, r = residual_norm(r.to(self.dtype), None, self.pre[0])[0], r
+        for i in range(len(self.blocks)):
+            u, r = residual_norm(block_out(i, u), r, self.pre[i + 1], post_weight=self.post[i],
+                                 scale=self.scale[i])
+        return u
+
+    def forward(self, tokens: torch.Tensor, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits [B, L, vocab] of whole sequences."""
+        return self.head(self._run(tokens, lambda i, u: self.blocks[i](u, lengths=lengths)))
+
+    def new_cache(self, pool: int) -> SelectiveCache:
+        dev = self.embedding.weight.device
+        return SelectiveCache(
+            [torch.zeros(pool, b.taps - 1, b.inner, dtype=self.dtype, device=dev)
+             for b in self.blocks],
+            [torch.zeros(pool, b.inner, b.state, device=dev) for b in self.blocks])
+
+    @torch.no_grad()
+    def prompt(self, tokens: torch.Tensor, cache: SelectiveCache, slots: torch.Tensor,
+               lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """A chunk [B, L] of prompts that go on from the states at ``slots``;
+        the logits [B, vocab] after each sequence's last token."""
+        at = slots.long()
+
+        def block_out(i: int, u: torch.Tensor) -> torch.Tensor:
+            out, conv, scan = self.blocks[i](u, cache.conv[i][at], cache.scan[i][at], lengths, True)
+            cache.conv[i][at], cache.scan[i][at] = conv, scan
+            return out
+
+        u = self._run(tokens, block_out)
+        if lengths is None:
+            return self.head(u[:, -1])
+        last = (lengths.long() - 1).clamp_(min=0)
+        return self.head(u[torch.arange(u.shape[0], device=u.device), last])
+
+    @torch.no_grad()
+    def step(self, tokens: torch.Tensor, cache: SelectiveCache,
+             slots: torch.Tensor | None = None) -> torch.Tensor:
+        """One token [B] of each sequence: logits [B, vocab]."""
+        return self.head(self._run(
+            tokens, lambda i, u: self.blocks[i].step(u, cache.conv[i], cache.scan[i], slots)))
+
+
+__all__ = ["SelectiveBlock", "SelectiveCache", "SelectiveModel"]
