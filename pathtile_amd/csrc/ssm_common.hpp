@@ -76,11 +76,9 @@ __device__ __forceinline__ void store_vec(__bf16* p, const float (&v)[V]) {
   }
 }
 
-// exp(v): the exponent in two terms, so that its rounding stays below 2^-24 of
-// the result for any |v|; a result below 2^-126 is 0.
-__device__ __forceinline__ float exp_f32(float v) {
-  return __builtin_amdgcn_exp2f(fmaf(v, 1.44269502162933349609375f, v * 1.92596303e-08f));
-}
+// exp(v). The exponent is rounded once, to 2^-24 |v| of the result; a result
+// below 2^-126 is 0.
+__device__ __forceinline__ float exp_f32(float v) { return __builtin_amdgcn_exp2f(v * kLog2E); }
 __device__ __forceinline__ float sigmoid_f32(float v) {
   return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v));
 }

@@ -36,9 +36,6 @@ __global__ __launch_bounds__(256) void scan_param_reduce_kernel(ScanArgs a, cons
   }
 }
 
-// States that the kernels hold: 16, 32 or 64.
-static int scan_index(int N) { return N <= 16 ? 0 : N <= 32 ? 1 : 2; }
-
 static int check_scan(const pt_scan_inputs* in, int L) {
   if (in->dtype != PT_F32 && in->dtype != PT_BF16) return PT_ERR_CONFIG;
   if (in->B < 0 || L < 1 || in->H < 1 || in->N < 1 || in->N > kScanMaxN || in->G < 1 || in->H % in->G)
@@ -47,6 +44,16 @@ static int check_scan(const pt_scan_inputs* in, int L) {
     return PT_ERR_SHAPE;
   if (in->B == 0) return PT_OK;
   return in->x && in->dt && in->a && in->b && in->c ? PT_OK : PT_ERR_NULL;
+}
+
+// Tiles of a chunk: sequences are taken in one piece where there is a workgroup
+// for each of 256 CUs, and otherwise in pieces of at least eight tiles, two to
+// a CU. Fewer than three pieces do not pay for the pass that they need first.
+static int scan_chunk_tiles(long long blocks, int ntiles) {
+  long long chunks = blocks >= 256 ? 1 : ssm_ceil(512, blocks);
+  if (chunks > ntiles / 8) chunks = ntiles / 8;
+  if (chunks < 3) chunks = 1;
+  return (int)ssm_ceil(ntiles, chunks);
 }
 
 static ScanArgs scan_args(const pt_scan_inputs* in) {
@@ -59,23 +66,22 @@ static ScanArgs scan_args(const pt_scan_inputs* in) {
   a.B = in->B, a.L = in->L, a.H = in->H, a.N = in->N, a.G = in->G, a.softplus = in->softplus;
   a.hg = in->H / in->G;
   a.blocks_g = (int)ssm_ceil(a.hg, kScanCh);
-  a.np = 16 << scan_index(in->N);
+  a.np = (int)ssm_ceil(in->N, 16) * 16;
   a.ntiles = (int)ssm_ceil(in->L, kScanTile);
+  a.chunk_tiles = scan_chunk_tiles((long long)a.B * a.blocks_g * a.G, a.ntiles);
+  a.chunks = (int)ssm_ceil(a.ntiles, a.chunk_tiles);
   return a;
 }
 
-// Whether the scalar loads can take B and C as they are: whole registers of
-// states, and pairs of BF16 on 4-byte boundaries.
-static bool scan_direct(const pt_scan_inputs* in) {
-  if (in->N != 16 << scan_index(in->N)) return false;
-  if (!ssm_aligned(in->b, 4) || !ssm_aligned(in->c, 4)) return false;
-  if (in->dtype == PT_F32) return true;
-  return ((in->b_batch | in->b_row | in->b_group | in->c_batch | in->c_row | in->c_group) & 1) == 0;
+// Floats that scan_bc_kernel writes, and those of the chunks' states and steps.
+static size_t scan_bc_floats(const ScanArgs& a) {
+  return ssm_round((size_t)a.B * a.G * a.ntiles * kScanTile * 2 * a.np);
 }
-
-static size_t scan_bc_floats(const pt_scan_inputs* in) {
-  return scan_direct(in) ? 0
-                         : ssm_round((size_t)in->B * in->L * in->G * 2 * (16 << scan_index(in->N)));
+static size_t scan_chunk_floats(const ScanArgs& a) {
+  return a.chunks > 1 ? ssm_round((size_t)a.B * a.chunks * (a.np + 1) * a.H) : 0;
+}
+static size_t scan_state_floats(const ScanArgs& a) {
+  return ssm_round((size_t)a.B * a.ntiles * a.np * a.H);
 }
 
 // Loads and stores of four channels: 16 bytes of FP32, 8 of BF16.
@@ -85,38 +91,29 @@ static bool scan_vector(const ScanArgs& a, int dtype, const void* const* ptrs, i
   return ok;
 }
 
-// B and C into the workspace where they are not taken as they are.
-static int scan_lay_out(const pt_scan_inputs* in, ScanArgs* a, float* ws, void* stream) {
-  if (scan_direct(in)) return PT_OK;
-  void* args[] = {a, &ws};
-  const void* fn = in->dtype == PT_F32 ? (const void*)&scan_bc_kernel<float>
-                                       : (const void*)&scan_bc_kernel<__bf16>;
-  const int st = ssm_launch(fn, ssm_ceil((long long)in->B * in->L * in->G * 2 * a->np, 256), 256,
-                            stream, args);
-  a->bm = ws, a->cm = ws + a->np;
-  a->b_group = a->c_group = 2 * a->np;
-  a->b_row = a->c_row = (long long)in->G * 2 * a->np;
-  a->b_batch = a->c_batch = a->b_row * in->L;
-  return st;
+static int scan_lay_out(const ScanArgs& a, int dtype, float* bc, void* stream) {
+  void* args[] = {const_cast<ScanArgs*>(&a), &bc};
+  const void* fn = dtype == PT_F32 ? (const void*)&scan_bc_kernel<float>
+                                   : (const void*)&scan_bc_kernel<__bf16>;
+  const long long lanes = (long long)a.B * a.G * (a.np / 4) * a.ntiles * kScanTile;
+  return ssm_launch(fn, ssm_ceil(lanes, 256), 256, stream, args);
 }
 
 struct ScanBwdLayout {
-  size_t bc, part_a, part_d, total;
+  size_t part_bc, part_a, part_d, total;
 };
-static ScanBwdLayout scan_bwd_layout(const pt_scan_inputs* in, const ScanArgs& a) {
+static ScanBwdLayout scan_bwd_layout(const ScanArgs& a) {
   ScanBwdLayout o;
-  o.bc = scan_bc_floats(in);
-  o.part_a = o.bc + ssm_round((size_t)a.blocks_g * a.G * a.B * a.L * 2 * a.np);
-  o.part_d = o.part_a + ssm_round((size_t)a.B * a.np * a.H);
-  o.total = (o.part_d + (size_t)a.B * 2 * a.H) * sizeof(float);
+  const size_t parts = (size_t)a.B * a.chunks;
+  o.part_bc = scan_chunk_floats(a);
+  o.part_a = o.part_bc + ssm_round((size_t)a.blocks_g * a.G * a.B * a.L * 2 * a.np);
+  o.part_d = o.part_a + ssm_round(parts * a.np * a.H);
+  o.total = (o.part_d + parts * 2 * a.H) * sizeof(float);
   return o;
 }
 
-static long long scan_blocks(const ScanArgs& a) { return (long long)a.B * a.blocks_g * a.G; }
-
-// [FP32; BF16; BF16 with B and C laid out as FP32]
-static int scan_types(const pt_scan_inputs* in) {
-  return in->dtype == PT_F32 ? 0 : scan_direct(in) ? 1 : 2;
+static long long scan_blocks(const ScanArgs& a) {
+  return (long long)a.B * a.chunks * a.blocks_g * a.G;
 }
 
 template <typename T, int PER>
@@ -134,9 +131,10 @@ int pt_selective_scan_sizes(const pt_scan_inputs* in, size_t* fwd_workspace, siz
   const int st = pt::check_scan(in, in->L);
   if (st != PT_OK) return st;
   const pt::ScanArgs a = pt::scan_args(in);
-  if (fwd_workspace) *fwd_workspace = pt::scan_bc_floats(in) * sizeof(float);
-  if (saved) *saved = (size_t)a.B * a.ntiles * a.np * a.H * sizeof(float);
-  if (bwd_workspace) *bwd_workspace = pt::scan_bwd_layout(in, a).total;
+  const size_t bc = pt::scan_bc_floats(a);
+  if (fwd_workspace) *fwd_workspace = (pt::scan_chunk_floats(a) + bc) * sizeof(float);
+  if (saved) *saved = (pt::scan_state_floats(a) + bc) * sizeof(float);
+  if (bwd_workspace) *bwd_workspace = pt::scan_bwd_layout(a).total;
   return PT_OK;
 }
 
@@ -147,16 +145,29 @@ int pt_selective_scan_fwd(const pt_scan_inputs* in, void* y, float* state_out, f
   if (st != PT_OK) return st;
   if (in->B == 0) return PT_OK;
   if (!y) return PT_ERR_NULL;
-  const size_t need = pt::scan_bc_floats(in) * sizeof(float);
-  if (need && (!workspace || workspace_bytes < need)) return PT_ERR_WORKSPACE;
-  pt::ScanFwdArgs f = {pt::scan_args(in), y, state_out, saved};
+  const pt::ScanArgs a = pt::scan_args(in);
+  float* ws = static_cast<float*>(workspace);
+  const size_t need = (pt::scan_chunk_floats(a) + pt::scan_bc_floats(a)) * sizeof(float);
+  if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
+  if (!pt::ssm_aligned(workspace, 64) || !pt::ssm_aligned(saved, 64)) return PT_ERR_ALIGN;
   const void* ptrs[] = {in->x, in->dt, y};
-  const bool vec = pt::scan_vector(f.s, in->dtype, ptrs, 3);
-  st = pt::scan_lay_out(in, &f.s, static_cast<float*>(workspace), stream);
+  const bool vec = pt::scan_vector(a, in->dtype, ptrs, 3);
+  const int type = in->dtype == PT_BF16, index = in->N > 16;
+  float* bc = saved ? saved + pt::scan_state_floats(a) : ws + pt::scan_chunk_floats(a);
+  st = pt::scan_lay_out(a, in->dtype, bc, stream);
   if (st != PT_OK) return st;
+  float* steps = ws + (size_t)a.B * a.chunks * a.np * a.H;
+  if (a.chunks > 1) {
+    pt::ScanChunkArgs c = {a, bc, nullptr, ws, steps};
+    void* args[] = {&c};
+    st = pt::ssm_launch((const void*)pt::kScanChunkFwd[type][index][vec], pt::scan_blocks(a),
+                        pt::kScanThreads, stream, args);
+    if (st != PT_OK) return st;
+  }
+  pt::ScanFwdArgs f = {a, bc, ws, steps, y, state_out, saved};
   void* args[] = {&f};
-  return pt::ssm_launch((const void*)pt::kScanFwd[pt::scan_types(in)][pt::scan_index(in->N)][vec],
-                        pt::scan_blocks(f.s), pt::kScanThreads, stream, args);
+  return pt::ssm_launch((const void*)pt::kScanFwd[type][index][vec], pt::scan_blocks(a),
+                        pt::kScanThreads, stream, args);
 }
 
 int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float* saved,
@@ -169,19 +180,28 @@ int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float*
   if (!ga) return PT_ERR_NULL;
   if (in->B > 0 && (!gy || !saved || !gx || !gdt || !gb || !gc)) return PT_ERR_NULL;
   pt::ScanArgs a = pt::scan_args(in);
-  const pt::ScanBwdLayout o = pt::scan_bwd_layout(in, a);
+  const pt::ScanBwdLayout o = pt::scan_bwd_layout(a);
   if (in->B > 0 && (!workspace || workspace_bytes < o.total)) return PT_ERR_WORKSPACE;
+  if (!pt::ssm_aligned(workspace, 64) || !pt::ssm_aligned(saved, 64)) return PT_ERR_ALIGN;
   float* ws = static_cast<float*>(workspace);
   const void* ptrs[] = {in->x, in->dt, gy, gx, gdt};
   const bool vec = pt::scan_vector(a, in->dtype, ptrs, 5);
-  float *part_bc = ws + o.bc, *part_a = ws + o.part_a, *part_d = ws + o.part_d;
+  const int type = in->dtype == PT_BF16, index = in->N > 16;
+  float *part_bc = ws + o.part_bc, *part_a = ws + o.part_a, *part_d = ws + o.part_d;
   if (in->B > 0) {
-    st = pt::scan_lay_out(in, &a, ws, stream);
-    if (st != PT_OK) return st;
-    pt::ScanBwdArgs f = {a, gy, saved, gstate_out, gx, gdt, gstate, part_bc, part_a, part_d};
+    const float* bc = saved + pt::scan_state_floats(a);
+    float* steps = ws + (size_t)a.B * a.chunks * a.np * a.H;
+    if (a.chunks > 1) {
+      pt::ScanChunkArgs c = {a, bc, gy, ws, steps};
+      void* args[] = {&c};
+      st = pt::ssm_launch((const void*)pt::kScanChunkBwd[type][index][vec], pt::scan_blocks(a),
+                          pt::kScanThreads, stream, args);
+      if (st != PT_OK) return st;
+    }
+    pt::ScanBwdArgs f = {a, bc, ws, steps, gy, saved, gstate_out, gx, gdt, gstate, part_bc, part_a, part_d};
     void* args[] = {&f};
-    st = pt::ssm_launch((const void*)pt::kScanBwd[pt::scan_types(in)][pt::scan_index(in->N)][vec],
-                        pt::scan_blocks(a), pt::kScanThreads, stream, args);
+    st = pt::ssm_launch((const void*)pt::kScanBwd[type][index][vec], pt::scan_blocks(a),
+                        pt::kScanThreads, stream, args);
     if (st != PT_OK) return st;
     const float* cpart = part_bc;
     void* bargs[] = {&a, &cpart, &gb, &gc};
@@ -190,7 +210,8 @@ int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float*
                         pt::ssm_ceil((long long)a.B * a.L * a.G * 2 * a.np, 256), 256, stream, bargs);
     if (st != PT_OK) return st;
   }
-  void* pargs[] = {&a, &part_a, &part_d, &ga, &gd, &gdt_bias, &a.B};
+  int parts = a.B * a.chunks;
+  void* pargs[] = {&a, &part_a, &part_d, &ga, &gd, &gdt_bias, &parts};
   return pt::ssm_launch((const void*)&pt::scan_param_reduce_kernel,
                         pt::ssm_ceil((long long)(a.np + 2) * a.H, 64), 256, stream, pargs);
 }

@@ -7,11 +7,12 @@
 // token and a group of channels, states are FP32.
 //
 // A workgroup owns 64 channels of one sequence, a lane each; its four waves
-// share the channels and split the states, so that B and C are the same for
-// all lanes of a wave and come through the scalar cache. Tokens go by tiles of
-// 16: every thread loads four channels of one token and puts d and d x into
-// LDS, the waves run the recurrence on them, and the same threads add the four
-// waves' parts of y.
+// share the channels and split 16 states by fours, so that B and C are the same
+// for all lanes of a wave and come through the scalar cache. More than 16
+// states take rounds of 16 over each tile, with the states of the other rounds
+// in LDS (MANY). Tokens go by tiles of 16: every thread loads four channels
+// of one token and puts d and d x into LDS, the waves run the recurrence on
+// them, and the same threads add the four waves' parts of y.
 
 #pragma once
 
@@ -38,6 +39,7 @@ struct ScanArgs {
   int hg, blocks_g;             // channels of a group; workgroups that cover them
   int np;                       // N rounded up to what the kernels hold
   int ntiles;                   // tiles of a sequence
+  int chunks, chunk_tiles;      // chunks that run side by side; tiles of one
 };
 
 __device__ __forceinline__ int scan_length(const ScanArgs& a, int b) {
@@ -48,46 +50,76 @@ __device__ __forceinline__ int scan_length(const ScanArgs& a, int b) {
 
 // softplus(v) = log(1 + e^v) and its derivative. log(u) e / (u - 1) with the
 // rounded u = 1 + e keeps the result's relative precision at small e, where
-// log(u) alone would lose it.
+// log(u) alone would lose it (3e-7 over e = 2^-24 .. 1). From 20 on it is v.
+// Selects of computed values, no branches: four of these interleave.
 __device__ __forceinline__ float softplus_f32(float v, float* grad) {
-  const float e = exp_f32(v > 20.0f ? 20.0f : v), u = 1.0f + e;  // a NaN stays one
+  const float w = v > 20.0f ? 20.0f : v;  // a NaN stays one
+  const float e = exp_f32(w), u = 1.0f + e, below = u - 1.0f;
   const float l = __builtin_amdgcn_logf(u) * kLn2;
-  *grad = v > 20.0f ? 1.0f : e * __builtin_amdgcn_rcpf(u);
-  return v > 20.0f ? v : u == 1.0f ? e : l * (e * __builtin_amdgcn_rcpf(u - 1.0f));
+  *grad = e * __builtin_amdgcn_rcpf(u);
+  const float r = l * (e * __builtin_amdgcn_rcpf(below)), small = below == 0.0f ? e : r;
+  return v > 20.0f ? v : small;
 }
 
-// N values that all lanes share, through the scalar cache.
-typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
-template <int NS>
-__device__ __forceinline__ void load_uniform(const float* p, float (&v)[NS]) {
+// B and C as the waves read them: for every four states and four tokens 32
+// floats that all lanes share, B[4] and C[4] of each token, in scalar
+// registers. [B, G, np / 4, 16 ntiles, 2, 4]; zeros from state N on and past a
+// sequence's end, so that a tile is always whole.
+constexpr int kScanGroup = 4;  // tokens of a scalar load
+typedef uint32_t u16s __attribute__((ext_vector_type(16)));
+typedef const __attribute__((address_space(4))) u16s* scalar_ptr;
+struct BcGroup {
+  u16s q[2];
+  __device__ __forceinline__ float b(int t, int i) const { return __uint_as_float(q[t >> 1][(t & 1) * 8 + i]); }
+  __device__ __forceinline__ float c(int t, int i) const { return __uint_as_float(q[t >> 1][(t & 1) * 8 + 4 + i]); }
+};
+__device__ __forceinline__ BcGroup load_group(const float* p) {
   scalar_ptr q = (scalar_ptr)(uintptr_t)p;
-#pragma unroll
-  for (int i = 0; i < NS; ++i) v[i] = __uint_as_float(q[i]);
+  return {q[0], q[1]};
 }
-template <int NS>
-__device__ __forceinline__ void load_uniform(const __bf16* p, float (&v)[NS]) {
-  scalar_ptr q = (scalar_ptr)(uintptr_t)p;
-#pragma unroll
-  for (int i = 0; i < NS; i += 2) {
-    const uint32_t u = q[i / 2];
-    v[i] = bf16_lo(u), v[i + 1] = bf16_hi(u);
-  }
-}
+// Scalar loads return in any order, so a wait is for all of them: the wait for
+// a group comes before the next one is asked for, and the group in between is
+// worked on while that is under way.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
+__device__ __forceinline__ void wait_groups() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0)
 
-// Four channels of one token, those below `n` (0 elsewhere).
-template <bool VEC, typename T>
-__device__ __forceinline__ void load_four(const T* p, int n, float (&v)[4]) {
+// Four channels of one token, those below `n` (0 elsewhere), as they are in
+// memory while they are under way.
+template <typename T, bool VEC>
+struct Four {
+  T v[4];
+};
+template <>
+struct Four<float, true> {
+  f4v v;
+};
+template <>
+struct Four<__bf16, true> {
+  u2v v;
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void fetch_four(const T* p, int n, Four<T, VEC>& f) {
   if constexpr (VEC) {
-    if (n > 0) {
-      load_vec<4>(p, v);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 0.0f;
+    f.v = {};
+    if (n > 0) f.v = *reinterpret_cast<const decltype(f.v)*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? load1(p + i) : 0.0f;
+    for (int i = 0; i < 4; ++i) f.v[i] = i < n ? p[i] : (T)0.0f;
   }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ float at_four(const Four<T, VEC>& f, int i) {
+  if constexpr (VEC && sizeof(T) == 2)
+    return i & 1 ? bf16_hi(f.v[i / 2]) : bf16_lo(f.v[i / 2]);
+  else
+    return (float)f.v[i];
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_four(const T* p, int n, float (&v)[4]) {
+  Four<T, VEC> f;
+  fetch_four(p, n, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = at_four(f, i);
 }
 template <bool VEC, typename T>
 __device__ __forceinline__ void store_four(T* p, int n, const float (&v)[4]) {
@@ -100,33 +132,42 @@ __device__ __forceinline__ void store_four(T* p, int n, const float (&v)[4]) {
   }
 }
 
-// B and C as FP32 [B, L, G, 2, np], zeros from state N on: for layouts that
-// the scalar loads cannot take as they are.
+// Four tokens of B and C for one token and four states a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(ScanArgs a, float* __restrict__ out) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = id / (2 * a.np);  // (b L + t) G + g
-  if (row >= (long long)a.B * a.L * a.G) return;
-  const int r = (int)(id - row * 2 * a.np), half = r / a.np, n = r - half * a.np;
-  const int g = (int)(row % a.G);
-  const long long bt = row / a.G;
-  const long long b = bt / a.L, t = bt - b * a.L;
-  float v = 0.0f;
-  if (n < a.N)
-    v = half ? load1(static_cast<const T*>(a.cm) + b * a.c_batch + t * a.c_row + (long long)g * a.c_group + n)
-             : load1(static_cast<const T*>(a.bm) + b * a.b_batch + t * a.b_row + (long long)g * a.b_group + n);
-  out[id] = v;
+  const int lp = a.ntiles * kScanTile, quads = a.np / 4;
+  const long long row = id / lp;  // (b G + g) quads + quad
+  if (row >= (long long)a.B * a.G * quads) return;
+  const int t = (int)(id - row * lp), w = (int)(row % quads), n = w * 4;
+  const long long bg = row / quads;
+  const int b = (int)(bg / a.G), g = (int)(bg - (long long)b * a.G);
+  f4v bv = {0.0f, 0.0f, 0.0f, 0.0f}, cv = bv;
+  if (t < scan_length(a, b)) {
+    const T* bp = static_cast<const T*>(a.bm) + b * a.b_batch + t * a.b_row + (long long)g * a.b_group + n;
+    const T* cp = static_cast<const T*>(a.cm) + b * a.c_batch + t * a.c_row + (long long)g * a.c_group + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) bv[i] = load1(bp + i), cv[i] = load1(cp + i);
+  }
+  f4v* o = reinterpret_cast<f4v*>(out + id * 8);
+  o[0] = bv, o[1] = cv;
 }
 
-// Where a workgroup works: blocks of channels are fastest.
+// Where a workgroup works: blocks of channels are fastest, then the chunks of
+// a sequence.
 struct ScanPlace {
   int blk, g, h0, nh, b;  // block, group, first channel, channels, sequence
+  int c, first, last;     // chunk; its tiles [first, last), of all tokens
 };
 __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t id) {
   ScanPlace p;
-  const int blocks = a.blocks_g * a.G;
-  p.b = (int)(id / (uint32_t)blocks);
-  p.blk = (int)(id - (uint32_t)p.b * blocks);
+  const uint32_t blocks = (uint32_t)(a.blocks_g * a.G), bc = id / blocks;
+  p.blk = (int)(id - bc * blocks);
+  p.b = (int)(bc / (uint32_t)a.chunks);
+  p.c = (int)(bc - (uint32_t)p.b * a.chunks);
+  p.first = p.c * a.chunk_tiles;
+  p.last = p.first + a.chunk_tiles < a.ntiles ? p.first + a.chunk_tiles : a.ntiles;
   p.g = p.blk / a.blocks_g;
   const int k = p.blk - p.g * a.blocks_g;
   p.h0 = p.g * a.hg + k * kScanCh;
@@ -134,30 +175,261 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t id) 
   return p;
 }
 
+// Rounds of 16 states over a tile; a lane's four states of one in memory: of
+// [.., H, N] as the caller has them, and of [.., np, H], coalesced, where the
+// kernels keep states for themselves.
+template <bool MANY>
+__device__ __forceinline__ int scan_rounds(const ScanArgs& a) {
+  return MANY ? a.np / 16 : 1;
+}
+__device__ __forceinline__ void load_states(const float* p, bool mine, const ScanArgs& a,
+                                            long long row, int r, int wave, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = (r * kScanWaves + wave) * 4 + i;
+    v[i] = p && mine && n < a.N ? p[row * a.N + n] : 0.0f;
+  }
+}
+__device__ __forceinline__ void store_states(float* p, bool mine, const ScanArgs& a, long long row,
+                                             int r, int wave, const float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = (r * kScanWaves + wave) * 4 + i;
+    if (p && mine && n < a.N) p[row * a.N + n] = v[i];
+  }
+}
+__device__ __forceinline__ long long state_at(const ScanArgs& a, long long row, int r, int wave, int h) {
+  return (row * a.np + (r * kScanWaves + wave) * 4) * a.H + h;
+}
+// Rows of A times log2 e, for exp2.
+__device__ __forceinline__ void load_rates(const ScanArgs& a, bool mine, int h, int r, int wave,
+                                           float (&v)[4]) {
+  load_states(a.a, mine, a, h, r, wave, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] *= kLog2E;
+}
+
+// Four values a lane of each round: in registers for one, in LDS for more.
+constexpr int kScanRounds = kScanMaxN / 16;
+template <bool MANY>
+struct Rounds;
+template <>
+struct Rounds<false> {
+  struct Lds {};
+  float v[4];
+  __device__ __forceinline__ Rounds(Lds&) {}
+  __device__ __forceinline__ void get(int, float (&o)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = v[i];
+  }
+  __device__ __forceinline__ void set(int, const float (&o)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = o[i];
+  }
+};
+template <>
+struct Rounds<true> {
+  struct Lds {
+    float v[kScanRounds][4][kScanThreads];
+  };
+  Lds& lds;
+  __device__ __forceinline__ Rounds(Lds& l) : lds(l) {}
+  __device__ __forceinline__ void get(int r, float (&o)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = lds.v[r][i][threadIdx.x];
+  }
+  __device__ __forceinline__ void set(int r, const float (&o)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds.v[r][i][threadIdx.x] = o[i];
+  }
+};
+
+// s of a round through the chunks [from, to), upwards or downwards.
+__device__ __forceinline__ void join_chunks(const ScanArgs& a, const float* states, const float* steps,
+                                            int b, int from, int to, int r, int wave, int h,
+                                            const float (&a2)[4], float (&s)[4]) {
+  const int way = from < to ? 1 : -1;
+#pragma unroll 4
+  for (int c = from; c != to; c += way) {
+    const long long row = (long long)b * a.chunks + c;
+    const float d = steps[row * a.H + h];
+    const float* p = states + state_at(a, row, r, wave, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      s[i] = fmaf(__builtin_amdgcn_exp2f(d * a2[i]), s[i], p[(long long)i * a.H]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// A sequence in chunks. Where sequences and channels alone leave the CUs
+// without work, the chunks of a sequence run side by side: this kernel first
+// gives each chunk's own state from a state of zero, s_c, and the sum D_c of
+// its steps; the scan of chunk c then starts from
+//   S_c = exp(A D_{c-1}) S_{c-1} + s_{c-1},  S_0 the first state.
+// REV is the same for the backward's q, from the last chunk to the first:
+//   q <- a (C gy + q).
+// ---------------------------------------------------------------------------
+struct ScanChunkArgs {
+  ScanArgs s;
+  const float* bc;
+  const void* gy;  // REV: [B, L, H] contiguous
+  float* states;   // [B, chunks, np, H]
+  float* steps;    // [B, chunks, H]
+};
+
+template <typename T, bool MANY, bool VEC, bool REV>
+__global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs f) {
+  constexpr int kGroups = kScanTile / kScanGroup;
+  __shared__ float2 du[2][kScanTile][kScanCh];
+  __shared__ typename Rounds<MANY>::Lds hold;
+  const ScanArgs& a = f.s;
+  const ScanPlace p = scan_place(a, blockIdx.x);
+  if (p.c == (REV ? 0 : a.chunks - 1)) return;  // no chunk starts from its state
+  const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool mine = lane < p.nh;
+  const int h = p.h0 + lane;
+  Rounds<MANY> states(hold);
+  float a2[4], steps = 0.0f;
+  const float zero[4] = {};
+  for (int r = 0; r < rounds; ++r) states.set(r, zero);
+  load_rates(a, mine, h, 0, wave, a2);
+
+  const int row = tid >> 4, c0 = (tid & 15) * 4, cn = p.nh - c0;
+  const T* xp = REV ? static_cast<const T*>(f.gy) + (long long)p.b * a.L * a.H
+                    : static_cast<const T*>(a.x) + (long long)p.b * a.x_batch;
+  const long long xrow = REV ? a.H : a.x_row;
+  xp += p.h0 + c0;
+  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
+  float bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
+  Four<T, VEC> xv, dv;
+  auto fetch = [&](int tile) {
+    const int t = tile * kScanTile + row;
+    const int n = t < len ? cn : 0;
+    fetch_four(xp + (n > 0 ? t * xrow : 0), n, xv);
+    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+  };
+  auto put = [&](int tile) {
+    const bool in = tile * kScanTile + row < len;
+    float d[4], g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i];
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &g);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = at_four(xv, i);
+      du[tile & 1][row][c0 + i] = in ? make_float2(d[i], REV ? x : d[i] * x) : make_float2(0.0f, 0.0f);
+    }
+  };
+  const int tiles = (len + kScanTile - 1) / kScanTile;
+  const int last = p.last < tiles ? p.last : tiles, n = last - p.first;
+  auto at = [&](int k) { return REV ? last - 1 - k : p.first + k; };
+  const size_t quad = (size_t)a.ntiles * kScanTile * 8;  // floats of four states
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
+  auto group_at = [&](int tile, int r, int g) {
+    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + (REV ? kGroups - 1 - g : g)) * kScanGroup * 8;
+  };
+  BcGroup next = {};
+  if (n > 0) {
+    next = load_group(group_at(at(0), 0, 0));
+    fetch(at(0));
+    put(at(0));
+    if (n > 1) fetch(at(1));
+  }
+  wait_loads();
+  __syncthreads();
+  for (int k = 0; k < n; ++k) {
+    const int tile = at(k);
+    float2 q[kScanTile];
+#pragma unroll
+    for (int t = 0; t < kScanTile; ++t) q[t] = du[tile & 1][t][lane];
+    for (int r = 0; r < rounds; ++r) {
+      float s[4], a3[4];
+      states.get(r, s);
+      if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        wait_groups();
+        const BcGroup now = next;
+        if (g + 1 < kGroups)
+          next = load_group(group_at(tile, r, g + 1));
+        else  // of the next round or tile; the last one's own again
+          next = load_group(r + 1 < rounds ? group_at(tile, r + 1, 0) : group_at(at(k + 1 < n ? k + 1 : k), 0, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int jj = 0; jj < kScanGroup; ++jj) {
+          const int j = REV ? kScanGroup - 1 - jj : jj;
+          const int t = (REV ? kGroups - 1 - g : g) * kScanGroup + j;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(q[t].x * a2[i]);
+            s[i] = REV ? e * fmaf(now.c(j, i), q[t].y, s[i]) : fmaf(e, s[i], q[t].y * now.b(j, i));
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      states.set(r, s);
+      if (MANY) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
+      }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kScanTile; ++t) sum += q[t].x;
+    steps += sum;
+    if (k + 1 < n) {
+      put(at(k + 1));
+      if (k + 2 < n) fetch(at(k + 2));
+    }
+    __syncthreads();
+  }
+  if (!mine) return;
+  const long long out = (long long)p.b * a.chunks + p.c;
+  for (int r = 0; r < rounds; ++r) {
+    float s[4];
+    states.get(r, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.states[state_at(a, out, r, wave, h) + (long long)i * a.H] = s[i];
+  }
+  if (wave == 0) f.steps[out * a.H + h] = steps;
+}
+
 struct ScanFwdArgs {
   ScanArgs s;
+  const float* bc;   // scan_bc_kernel's
+  const float *chunk_states, *chunk_steps;  // scan_chunk_kernel's (chunks > 1)
   void* y;           // [B, L, H] contiguous
   float* state_out;  // [B, H, N] or null
   float* saved;      // [B, ntiles, np, H]: the state before each tile, or null
 };
 
-template <typename T, typename BCT, int NS, bool VEC>
+template <typename T, bool MANY, bool VEC>
 __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
+  constexpr int kGroups = kScanTile / kScanGroup;
   __shared__ float2 du[2][kScanTile][kScanCh];
   __shared__ float yp[2][kScanWaves][kScanTile][kScanCh];
+  __shared__ typename Rounds<MANY>::Lds hold;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
-  const int len = scan_length(a, p.b);
+  const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
-  const int h = p.h0 + lane, n0 = wave * NS;
+  const int h = p.h0 + lane;
 
-  float a2[NS], s[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const bool in = mine && n0 + i < a.N;
-    a2[i] = in ? a.a[(long long)h * a.N + n0 + i] * kLog2E : 0.0f;
-    s[i] = in && a.state ? a.state[((long long)p.b * a.H + h) * a.N + n0 + i] : 0.0f;
+  Rounds<MANY> states(hold);
+  float a2[4];
+  for (int r = rounds - 1; r >= 0; --r) {
+    float s[4];
+    load_rates(a, mine, h, r, wave, a2);
+    load_states(a.state, mine, a, (long long)p.b * a.H + h, r, wave, s);
+    if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, 0, p.c, r, wave, h, a2, s);
+    states.set(r, s);
   }
 
   // Loading and storing: token tid / 16 of a tile, four channels.
@@ -165,71 +437,99 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
   const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
   T* yo = static_cast<T*>(f.y) + (long long)p.b * a.L * a.H + p.h0 + c0;
-  float bias[4], dskip[4], xv[4], dv[4], xk[4];
+  float bias[4], dskip[4], xk[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
     dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
   }
+  Four<T, VEC> xv, dv;
   auto fetch = [&](int tile) {
     const int t = tile * kScanTile + row;
     const int n = t < len ? cn : 0;
-    load_four<VEC>(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    load_four<VEC>(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    fetch_four(xp + (n > 0 ? t * a.x_row : 0), n, xv);
+    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
   };
   auto put = [&](int tile) {
     const bool in = tile * kScanTile + row < len;
+    float d[4], g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float g, d = dv[i] + bias[i];
-      if (a.softplus) d = softplus_f32(d, &g);
-      xk[i] = xv[i];
-      du[tile & 1][row][c0 + i] = in ? make_float2(d, d * xv[i]) : make_float2(0.0f, 0.0f);
+    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i], xk[i] = at_four(xv, i);
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &g);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      du[tile & 1][row][c0 + i] = in ? make_float2(d[i], d[i] * xk[i]) : make_float2(0.0f, 0.0f);
   };
 
   const int tiles = (len + kScanTile - 1) / kScanTile;
-  const BCT* bp = static_cast<const BCT*>(a.bm) + p.b * a.b_batch + (long long)p.g * a.b_group + n0;
-  const BCT* cp = static_cast<const BCT*>(a.cm) + p.b * a.c_batch + (long long)p.g * a.c_group + n0;
-  if (tiles > 0) {
-    fetch(0);
-    put(0);
-    if (tiles > 1) fetch(1);
+  const int last = p.last < tiles ? p.last : tiles;
+  const size_t quad = (size_t)a.ntiles * kScanTile * 8;  // floats of four states
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
+  auto group_at = [&](int tile, int r, int g) {
+    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + g) * kScanGroup * 8;
+  };
+  BcGroup next = {};
+  if (p.first < last) {
+    next = load_group(group_at(p.first, 0, 0));
+    fetch(p.first);
+    put(p.first);
+    if (p.first + 1 < last) fetch(p.first + 1);
   }
+  wait_loads();
   __syncthreads();
-  for (int tile = 0; tile < tiles; ++tile) {
-    if (f.saved && mine) {
-      float* sp = f.saved + (((long long)p.b * a.ntiles + tile) * a.np + n0) * a.H + h;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) sp[(long long)i * a.H] = s[i];
-    }
-    const int count = len - tile * kScanTile < kScanTile ? len - tile * kScanTile : kScanTile;
+  for (int tile = p.first; tile < last; ++tile) {
     const int buf = tile & 1;
-    auto step = [&](int t) {
-      const float2 q = du[buf][t][lane];
-      float bv[NS], cv[NS], y = 0.0f;
-      load_uniform<NS>(bp, bv);
-      load_uniform<NS>(cp, cv);
-      bp += a.b_row, cp += a.c_row;
+    float2 q[kScanTile];
+    float y[kScanTile];
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        s[i] = fmaf(__builtin_amdgcn_exp2f(q.x * a2[i]), s[i], q.y * bv[i]);
-        y = fmaf(cv[i], s[i], y);
+    for (int t = 0; t < kScanTile; ++t) q[t] = du[buf][t][lane], y[t] = 0.0f;
+    for (int r = 0; r < rounds; ++r) {
+      float s[4], a3[4];
+      states.get(r, s);
+      if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
+      if (f.saved && mine) {
+        float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sp[(long long)i * a.H] = s[i];
       }
-      yp[buf][wave][t][lane] = y;
-    };
-    if (count == kScanTile) {
-#pragma unroll 4
-      for (int t = 0; t < kScanTile; ++t) step(t);
-    } else {
-      for (int t = 0; t < count; ++t) step(t);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        wait_groups();
+        const BcGroup now = next;
+        if (g + 1 < kGroups)
+          next = load_group(group_at(tile, r, g + 1));
+        else  // of the next round or tile; the last one's own again
+          next = load_group(r + 1 < rounds ? group_at(tile, r + 1, 0)
+                                           : group_at(tile + 1 < last ? tile + 1 : tile, 0, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kScanGroup; ++j) {
+          const int t = g * kScanGroup + j;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[i] = fmaf(__builtin_amdgcn_exp2f(q[t].x * a2[i]), s[i], q[t].y * now.b(j, i));
+            y[t] = fmaf(now.c(j, i), s[i], y[t]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      states.set(r, s);
+      if (MANY) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
+      }
     }
+#pragma unroll
+    for (int t = 0; t < kScanTile; ++t) yp[buf][wave][t][lane] = y[t];
     float xr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) xr[i] = xk[i];
-    if (tile + 1 < tiles) {
+    if (tile + 1 < last) {
       put(tile + 1);
-      if (tile + 2 < tiles) fetch(tile + 2);
+      if (tile + 2 < last) fetch(tile + 2);
     }
     __syncthreads();
     const int t = tile * kScanTile + row;
@@ -237,21 +537,22 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
       float out[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float y = dskip[i] * xr[i];
+        float v = dskip[i] * xr[i];
 #pragma unroll
-        for (int w = 0; w < kScanWaves; ++w) y += yp[buf][w][row][c0 + i];
-        out[i] = row < count ? y : 0.0f;
+        for (int w = 0; w < kScanWaves; ++w) v += yp[buf][w][row][c0 + i];
+        out[i] = t < len ? v : 0.0f;
       }
       store_four<VEC>(yo + (long long)t * a.H, cn, out);
     }
   }
   const float zero[4] = {};
-  for (int t = tiles * kScanTile + row; t < a.L; t += kScanTile)
-    store_four<VEC>(yo + (long long)t * a.H, cn, zero);
-  if (f.state_out && mine) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (n0 + i < a.N) f.state_out[((long long)p.b * a.H + h) * a.N + n0 + i] = s[i];
+  for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile)
+    if (tile * kScanTile + row < a.L) store_four<VEC>(yo + (long long)(tile * kScanTile + row) * a.H, cn, zero);
+  if (p.c < a.chunks - 1) return;
+  for (int r = 0; r < rounds; ++r) {
+    float s[4];
+    states.get(r, s);
+    store_states(f.state_out, mine, a, (long long)p.b * a.H + h, r, wave, s);
   }
 }
 
@@ -264,22 +565,23 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 // runs the tile forward again from the state saved before it, with a and s of
 // all 16 tokens in registers, then backward. Sums over the states go through
 // LDS as y does; sums over the channels are butterflies over the lanes that
-// halve the number of values at each level, so that a value costs about two
-// instructions, and leave one (token, state) in each lane.
+// halve the number of values at each level and leave one (token, state) in
+// each lane: 126 folds for the 128 values of a wave's round.
 // ---------------------------------------------------------------------------
 struct ScanBwdArgs {
   ScanArgs s;
+  const float* bc;
+  const float *chunk_states, *chunk_steps;
   const void* gy;           // [B, L, H] contiguous
   const float* saved;       // of the forward
   const float* gstate_out;  // gradient of the final state [B, H, N], or null
   void *gx, *gdt;           // [B, L, H] contiguous
   float* gstate;            // [B, H, N] or null
   float* part_bc;           // [blocks][B][L][2][np]
-  float* part_a;            // [B][np][H]
-  float* part_d;            // [B][2][H]: dD, ddt_bias
+  float* part_a;            // [B chunks][np][H]
+  float* part_d;            // [B chunks][2][H]: dD, ddt_bias
 };
 
-typedef uint32_t u2s __attribute__((ext_vector_type(2)));
 // (lanes 0-31: u + u of lanes 32-63; lanes 32-63: the same of v)
 __device__ __forceinline__ float fold32(float u, float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(u), __float_as_uint(v), false, false);
@@ -298,30 +600,38 @@ __device__ __forceinline__ float fold_row(float u, float v, bool bit) {
 }
 constexpr int kDppRor8 = 0x128, kDppHalfMirror = 0x141, kDppXor2 = 0x4e, kDppXor1 = 0xb1;
 
-template <typename T, typename BCT, int R, bool VEC>
-__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdArgs f) {
-  constexpr int NS = 4;  // states of a wave in a round; R rounds
+template <typename T, bool MANY, bool VEC>
+__global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f) {
+  constexpr int kGroups = kScanTile / kScanGroup;
   __shared__ float2 du[kScanTile][kScanCh];
   __shared__ float gys[kScanTile][kScanCh];
   __shared__ float p1[kScanWaves][kScanTile][kScanCh], p2[kScanWaves][kScanTile][kScanCh];
+  __shared__ typename Rounds<MANY>::Lds hold_q, hold_a;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
-  const int len = scan_length(a, p.b);
+  const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
   const int h = p.h0 + lane;
+  const int tiles = (len + kScanTile - 1) / kScanTile;
+  const int last = p.last < tiles ? p.last : tiles;
 
-  float a2[R][NS], q[R][NS], ga[R][NS];
+  Rounds<MANY> qs(hold_q), gas(hold_a);
+  const float zero[4] = {};
+  float a2[4], s0[4];  // of the round at hand
+  auto load_saved = [&](int tile, int r, float(&v)[4]) {
+    const float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int n = (r * kScanWaves + wave) * NS + i;
-      const bool in = mine && n < a.N;
-      a2[r][i] = in ? a.a[(long long)h * a.N + n] * kLog2E : 0.0f;
-      q[r][i] = in && f.gstate_out ? f.gstate_out[((long long)p.b * a.H + h) * a.N + n] : 0.0f;
-      ga[r][i] = 0.0f;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = mine ? sp[(long long)i * a.H] : 0.0f;
+  };
+  for (int r = rounds - 1; r >= 0; --r) {
+    float q[4];
+    load_rates(a, mine, h, r, wave, a2);
+    load_states(f.gstate_out, mine, a, (long long)p.b * a.H + h, r, wave, q);
+    if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, a.chunks - 1, p.c, r, wave, h, a2, q);
+    qs.set(r, q);
+    gas.set(r, zero);
+  }
 
   const int row = tid >> 4, c0 = (tid & 15) * 4, cn = p.nh - c0;
   const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
@@ -336,103 +646,131 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdArgs f) {
     bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
     dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
   }
-  const int tiles = (len + kScanTile - 1) / kScanTile;
-  const float zero[4] = {};
-  for (int t = tiles * kScanTile + row; t < a.L; t += kScanTile) {
+  for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile) {
+    const int t = tile * kScanTile + row;
+    if (t >= a.L) continue;
     store_four<VEC>(gxp + (long long)t * a.H, cn, zero);
     store_four<VEC>(gdp + (long long)t * a.H, cn, zero);
   }
-  float xv[4], dv[4], gv[4];
+  Four<T, VEC> xv, dv, gv;
   auto fetch = [&](int tile) {
     const int t = tile * kScanTile + row;
     const int n = t < len ? cn : 0;
-    load_four<VEC>(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    load_four<VEC>(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
-    load_four<VEC>(gp + (n > 0 ? (long long)t * a.H : 0), n, gv);
+    fetch_four(xp + (n > 0 ? t * a.x_row : 0), n, xv);
+    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    fetch_four(gp + (n > 0 ? (long long)t * a.H : 0), n, gv);
   };
-  if (tiles > 0) fetch(tiles - 1);
-  for (int tile = tiles - 1; tile >= 0; --tile) {
-    const int t0 = tile * kScanTile, count = len - t0 < kScanTile ? len - t0 : kScanTile;
-    float x[4], d[4], sg[4], gy[4];
+  const size_t quad = (size_t)a.ntiles * kScanTile * 8;
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
+  auto group_at = [&](int tile, int r, int g) {
+    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + g) * kScanGroup * 8;
+  };
+  BcGroup next = {};
+  if (p.first < last) {
+    next = load_group(group_at(last - 1, 0, 0));
+    fetch(last - 1);
+    load_saved(last - 1, 0, s0);
+  }
+  wait_loads();
+  for (int tile = last - 1; tile >= p.first; --tile) {
+    const int t0 = tile * kScanTile;
+    const bool in = t0 + row < len;  // tokens past the end change nothing
+    float d[4], sg[4];
+    Four<T, VEC> xk = xv, gk = gv;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i], sg[i] = 1.0f;
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &sg[i]);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[i] = xv[i], gy[i] = gv[i], sg[i] = 1.0f, d[i] = dv[i] + bias[i];
-      if (a.softplus) d[i] = softplus_f32(d[i], &sg[i]);
-      du[row][c0 + i] = row < count ? make_float2(d[i], d[i] * x[i]) : make_float2(0.0f, 0.0f);
-      gys[row][c0 + i] = gy[i];
+      du[row][c0 + i] = in ? make_float2(d[i], d[i] * at_four(xk, i)) : make_float2(0.0f, 0.0f);
+      gys[row][c0 + i] = in ? at_four(gk, i) : 0.0f;
     }
-    if (tile > 0) fetch(tile - 1);
+    if (tile > p.first) fetch(tile - 1);
     __syncthreads();
-    float s1[R > 1 ? kScanTile : 1], s2[R > 1 ? kScanTile : 1];
+    for (int r = 0; r < rounds; ++r) {
+      float s[kScanTile + 1][4], e[kScanTile][4], q[4], a3[4];
+      const bool more = r + 1 < rounds;
+      const int tile2 = more ? tile : tile > p.first ? tile - 1 : tile, r2 = more ? r + 1 : 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int n0 = (r * kScanWaves + wave) * NS;
-      const BCT* bp = static_cast<const BCT*>(a.bm) + p.b * a.b_batch + t0 * a.b_row +
-                      (long long)p.g * a.b_group + n0;
-      const BCT* cp = static_cast<const BCT*>(a.cm) + p.b * a.c_batch + t0 * a.c_row +
-                      (long long)p.g * a.c_group + n0;
-      const float* sp = f.saved + (((long long)p.b * a.ntiles + tile) * a.np + n0) * a.H + h;
-      float s[kScanTile + 1][NS], e[kScanTile][NS];
+      for (int i = 0; i < 4; ++i) s[0][i] = s0[i];
+      load_saved(tile2, r2, s0);
+      if (MANY) load_rates(a, mine, h, r2, wave, a3);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[0][i] = mine ? sp[(long long)i * a.H] : 0.0f;
+      for (int g = 0; g < kGroups; ++g) {
+        float2 w[kScanGroup];
 #pragma unroll
-      for (int t = 0; t < kScanTile; ++t) {
-        if (t < count) {
-          const float2 w = du[t][lane];
-          float bv[NS];
-          load_uniform<NS>(bp + t * a.b_row, bv);
+        for (int j = 0; j < kScanGroup; ++j) w[j] = du[g * kScanGroup + j][lane];
+        wait_groups();
+        const BcGroup now = next;
+        // the last group is also the first one on the way back
+        if (g + 1 < kGroups) next = load_group(group_at(tile, r, g + 1));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            e[t][i] = __builtin_amdgcn_exp2f(w.x * a2[r][i]);
-            s[t + 1][i] = fmaf(e[t][i], s[t][i], w.y * bv[i]);
+        for (int j = 0; j < kScanGroup; ++j) {
+          const int t = g * kScanGroup + j;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[t][i] = __builtin_amdgcn_exp2f(w[j].x * a2[i]);
+            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * now.b(j, i));
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      float rb[kScanTile], rc[kScanTile], gat[NS] = {};
+      float rb[kScanTile], rc[kScanTile], ga[4] = {};
+      qs.get(r, q);
 #pragma unroll
-      for (int t = kScanTile - 1; t >= 0; --t) {
-        rb[t] = rc[t] = 0.0f;
-        if (t < count) {
-          const float2 w = du[t][lane];
-          const float gyt = gys[t][lane];
-          float bv[NS], cv[NS], vb[NS], vc[NS], u1 = 0.0f, u2 = 0.0f;
-          load_uniform<NS>(bp + t * a.b_row, bv);
-          load_uniform<NS>(cp + t * a.c_row, cv);
+      for (int g = kGroups - 1; g >= 0; --g) {
+        float2 w[kScanGroup];
+        float gyt[kScanGroup], o1[kScanGroup], o2[kScanGroup];
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            const float g = fmaf(cv[i], gyt, q[r][i]);
-            u1 = fmaf(g, bv[i], u1);
-            vb[i] = g * w.y;
-            vc[i] = gyt * s[t + 1][i];
-            q[r][i] = g * e[t][i];
-            const float k = q[r][i] * s[t][i];
-            u2 = fmaf(k, a2[r][i], u2);
-            gat[i] = fmaf(k, w.x, gat[i]);
+        for (int j = 0; j < kScanGroup; ++j) {
+          const int t = g * kScanGroup + j;
+          w[j] = du[t][lane], gyt[j] = gys[t][lane];
+          o1[j] = o2[j] = 0.0f;
+          if (MANY && r > 0) o1[j] = p1[wave][t][lane], o2[j] = p2[wave][t][lane];
+        }
+        wait_groups();
+        const BcGroup now = next;
+        next = load_group(g > 0 ? group_at(tile, r, g - 1) : group_at(tile2, r2, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = kScanGroup - 1; j >= 0; --j) {
+          const int t = g * kScanGroup + j;
+          float vb[4], vc[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float G = fmaf(now.c(j, i), gyt[j], q[i]);
+            o1[j] = fmaf(now.b(j, i), G, o1[j]);
+            vb[i] = G * w[j].y;
+            vc[i] = gyt[j] * s[t + 1][i];
+            q[i] = G * e[t][i];
+            const float k = q[i] * s[t][i];
+            o2[j] = fmaf(k, a2[i], o2[j]);
+            ga[i] = fmaf(k, w[j].x, ga[i]);
           }
           rb[t] = fold16(fold32(vb[0], vb[2]), fold32(vb[1], vb[3]));
           rc[t] = fold16(fold32(vc[0], vc[2]), fold32(vc[1], vc[3]));
-          if constexpr (R > 1) {
-            s1[t] = r == 0 ? u1 : s1[t] + u1;
-            s2[t] = r == 0 ? u2 : s2[t] + u2;
+          p1[wave][t][lane] = o1[j];
+          p2[wave][t][lane] = o2[j];
+          if (t < 8) {
+            rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 8], lane & 8);
+            rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 8], lane & 8);
           }
-          if (r == R - 1) {
-            p1[wave][t][lane] = R > 1 ? s1[R > 1 ? t : 0] : u1;
-            p2[wave][t][lane] = R > 1 ? s2[R > 1 ? t : 0] : u2;
+          if (t < 4) {
+            rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 4], lane & 4);
+            rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 4], lane & 4);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      qs.set(r, q);
+      gas.get(r, q);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) ga[r][i] += gat[i];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 8], lane & 8);
-        rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 8], lane & 8);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 4], lane & 4);
-        rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 4], lane & 4);
-      }
+      for (int i = 0; i < 4; ++i) ga[i] += q[i];
+      gas.set(r, ga);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         rb[t] = fold_row<kDppXor2>(rb[t], rb[t + 2], lane & 2);
@@ -443,9 +781,14 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdArgs f) {
       // lane: token lane % 16, state lane / 16
       const int t = t0 + (lane & 15);
       if (t < len) {
-        float* bc = f.part_bc + (((long long)p.blk * a.B + p.b) * a.L + t) * 2 * a.np + n0 + (lane >> 4);
-        bc[0] = rb[0];
-        bc[a.np] = rc[0];
+        float* o = f.part_bc + (((long long)p.blk * a.B + p.b) * a.L + t) * 2 * a.np +
+                   (r * kScanWaves + wave) * 4 + (lane >> 4);
+        o[0] = rb[0];
+        o[a.np] = rc[0];
+      }
+      if (MANY) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
       }
     }
     __syncthreads();
@@ -457,36 +800,36 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdArgs f) {
         float g1 = 0.0f, g2 = 0.0f;
 #pragma unroll
         for (int w = 0; w < kScanWaves; ++w) g1 += p1[w][row][c0 + i], g2 += p2[w][row][c0 + i];
-        ox[i] = od[i] = 0.0f;
-        if (row < count) {
-          ox[i] = fmaf(d[i], g1, dskip[i] * gy[i]);
-          od[i] = fmaf(x[i], g1, kLn2 * g2) * sg[i];
-          gd[i] = fmaf(gy[i], x[i], gd[i]);
-          gbias[i] += od[i];
-        }
+        const float x = at_four(xk, i), gy = at_four(gk, i);  // 0 past the end
+        ox[i] = in ? fmaf(d[i], g1, dskip[i] * gy) : 0.0f;
+        od[i] = in ? fmaf(x, g1, kLn2 * g2) * sg[i] : 0.0f;
+        gd[i] = fmaf(gy, x, gd[i]);
+        gbias[i] += od[i];
       }
       store_four<VEC>(gxp + (long long)t * a.H, cn, ox);
       store_four<VEC>(gdp + (long long)t * a.H, cn, od);
     }
     __syncthreads();
   }
+  const long long part = (long long)p.b * a.chunks + p.c;
+  for (int r = 0; r < rounds; ++r) {
+    float v[4];
+    gas.get(r, v);
+    if (mine) {
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int n = (r * kScanWaves + wave) * NS + i;
-      if (!mine) continue;
-      f.part_a[((long long)p.b * a.np + n) * a.H + h] = ga[r][i];
-      if (f.gstate && n < a.N) f.gstate[((long long)p.b * a.H + h) * a.N + n] = q[r][i];
+      for (int i = 0; i < 4; ++i) f.part_a[state_at(a, part, r, wave, h) + (long long)i * a.H] = v[i];
     }
+    qs.get(r, v);
+    if (p.c == 0) store_states(f.gstate, mine, a, (long long)p.b * a.H + h, r, wave, v);
+  }
   // The sums over the tokens of a tile's rows.
-  p1[0][row][c0] = gd[0], p1[0][row][c0 + 1] = gd[1], p1[0][row][c0 + 2] = gd[2], p1[0][row][c0 + 3] = gd[3];
-  p2[0][row][c0] = gbias[0], p2[0][row][c0 + 1] = gbias[1], p2[0][row][c0 + 2] = gbias[2], p2[0][row][c0 + 3] = gbias[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p1[0][row][c0 + i] = gd[i], p2[0][row][c0 + i] = gbias[i];
   __syncthreads();
   if (tid < 2 * kScanCh && mine) {
     float v = 0.0f;
     for (int t = 0; t < kScanTile; ++t) v += wave ? p2[0][t][lane] : p1[0][t][lane];
-    f.part_d[((long long)p.b * 2 + wave) * a.H + h] = v;
+    f.part_d[(part * 2 + wave) * a.H + h] = v;
   }
 }
 

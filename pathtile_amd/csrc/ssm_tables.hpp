@@ -6,11 +6,15 @@ namespace pt {
 
 struct ScanFwdArgs;
 struct ScanBwdArgs;
+struct ScanChunkArgs;
 using ScanFwdFn = void (*)(ScanFwdArgs);
 using ScanBwdFn = void (*)(ScanBwdArgs);
+using ScanChunkFn = void (*)(ScanChunkArgs);
 
-// [FP32; BF16; BF16 with B and C as FP32][16, 32, 64 states][single, vector]
-extern const ScanFwdFn kScanFwd[3][3][2];
-extern const ScanBwdFn kScanBwd[3][3][2];
+// [FP32, BF16][up to 16 states, more][single, vector loads]
+extern const ScanFwdFn kScanFwd[2][2][2];
+extern const ScanBwdFn kScanBwd[2][2][2];
+extern const ScanChunkFn kScanChunkFwd[2][2][2];
+extern const ScanChunkFn kScanChunkBwd[2][2][2];
 
 }  // namespace pt
