@@ -84,10 +84,10 @@ static size_t scan_state_floats(const ScanArgs& a) {
   return ssm_round((size_t)a.B * a.ntiles * a.np * a.H);
 }
 
-// Loads and stores of four channels: 16 bytes of FP32, 8 of BF16.
+// Loads and stores of two channels: 8 bytes of FP32, 4 of BF16.
 static bool scan_vector(const ScanArgs& a, int dtype, const void* const* ptrs, int n) {
-  bool ok = a.hg % 4 == 0 && ((a.x_batch | a.x_row | a.dt_batch | a.dt_row) & 3) == 0;
-  for (int i = 0; i < n; ++i) ok = ok && ssm_aligned(ptrs[i], dtype == PT_F32 ? 16 : 8);
+  bool ok = a.hg % kScanCols == 0 && ((a.x_batch | a.x_row | a.dt_batch | a.dt_row) & (kScanCols - 1)) == 0;
+  for (int i = 0; i < n; ++i) ok = ok && ssm_aligned(ptrs[i], dtype == PT_F32 ? 8 : 4);
   return ok;
 }
 
@@ -95,7 +95,7 @@ static int scan_lay_out(const ScanArgs& a, int dtype, float* bc, void* stream) {
   void* args[] = {const_cast<ScanArgs*>(&a), &bc};
   const void* fn = dtype == PT_F32 ? (const void*)&scan_bc_kernel<float>
                                    : (const void*)&scan_bc_kernel<__bf16>;
-  const long long lanes = (long long)a.B * a.G * (a.np / 4) * a.ntiles * kScanTile;
+  const long long lanes = (long long)a.B * a.G * (a.np / 2) * a.ntiles * kScanTile;
   return ssm_launch(fn, ssm_ceil(lanes, 256), 256, stream, args);
 }
 

@@ -6,13 +6,13 @@
 // for each sequence b and channel h, over its tokens; B and C belong to a
 // token and a group of channels, states are FP32.
 //
-// A workgroup owns 64 channels of one sequence, a lane each; its four waves
-// share the channels and split 16 states by fours, so that B and C are the same
+// A workgroup owns 64 channels of one sequence, a lane each; its eight waves
+// share the channels and split 16 states by twos, so that B and C are the same
 // for all lanes of a wave and come through the scalar cache. More than 16
 // states take rounds of 16 over each tile, with the states of the other rounds
-// in LDS (MANY). Tokens go by tiles of 16: every thread loads four channels
-// of one token and puts d and d x into LDS, the waves run the recurrence on
-// them, and the same threads add the four waves' parts of y.
+// in LDS (MANY). Tokens go by tiles of 16: every thread loads two channels of
+// one token and puts d and d x into LDS, the waves run the recurrence on them,
+// and the same threads add the eight waves' parts of y.
 
 #pragma once
 
@@ -22,8 +22,10 @@ namespace pt {
 
 constexpr int kScanTile = 16;      // tokens between two barriers, and between two saved states
 constexpr int kScanCh = 64;        // channels of a workgroup
-constexpr int kScanWaves = 4;
-constexpr int kScanThreads = 256;
+constexpr int kScanWaves = 8;
+constexpr int kScanStates = 2;     // of a wave: 16 a round
+constexpr int kScanThreads = 512;
+constexpr int kScanCols = 2;       // channels of a token that a thread loads and stores
 constexpr int kScanMaxN = 64;
 
 struct ScanArgs {
@@ -61,21 +63,30 @@ __device__ __forceinline__ float softplus_f32(float v, float* grad) {
   return v > 20.0f ? v : small;
 }
 
-// B and C as the waves read them: for every four states and four tokens 32
-// floats that all lanes share, B[4] and C[4] of each token, in scalar
-// registers. [B, G, np / 4, 16 ntiles, 2, 4]; zeros from state N on and past a
+// B and C as the waves read them: for every two states and eight tokens 16
+// floats B[8][2] and 16 of C that all lanes share, in scalar registers.
+// [B, G, np / 2, 2 ntiles, 2, 8, 2]; zeros from state N on and past a
 // sequence's end, so that a tile is always whole.
-constexpr int kScanGroup = 4;  // tokens of a scalar load
+constexpr int kScanGroup = 8;  // tokens of a scalar load
 typedef uint32_t u16s __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(4))) u16s* scalar_ptr;
+__device__ __forceinline__ u16s load_uniform(const float* p) { return *(scalar_ptr)(uintptr_t)p; }
+__device__ __forceinline__ float uniform_at(const u16s& q, int t, int i) {
+  return __uint_as_float(q[t * 2 + i]);
+}
 struct BcGroup {
-  u16s q[2];
-  __device__ __forceinline__ float b(int t, int i) const { return __uint_as_float(q[t >> 1][(t & 1) * 8 + i]); }
-  __device__ __forceinline__ float c(int t, int i) const { return __uint_as_float(q[t >> 1][(t & 1) * 8 + 4 + i]); }
+  u16s bq, cq;
+  __device__ __forceinline__ float b(int t, int i) const { return uniform_at(bq, t, i); }
+  __device__ __forceinline__ float c(int t, int i) const { return uniform_at(cq, t, i); }
 };
 __device__ __forceinline__ BcGroup load_group(const float* p) {
-  scalar_ptr q = (scalar_ptr)(uintptr_t)p;
-  return {q[0], q[1]};
+  return {load_uniform(p), load_uniform(p + 16)};
+}
+// Keeps what led to these values before what follows.
+template <int N>
+__device__ __forceinline__ void pin(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 // Scalar loads return in any order, so a wait is for all of them: the wait for
 // a group comes before the next one is asked for, and the group in between is
@@ -83,75 +94,84 @@ __device__ __forceinline__ BcGroup load_group(const float* p) {
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
 __device__ __forceinline__ void wait_groups() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0)
 
-// Four channels of one token, those below `n` (0 elsewhere), as they are in
-// memory while they are under way.
-template <typename T, bool VEC>
-struct Four {
-  T v[4];
+// V neighbouring values, those below `n` (0 elsewhere), as they are in memory
+// while they are under way.
+template <typename T, int V, bool VEC>
+struct Few {
+  T v[V];
 };
-template <>
-struct Four<float, true> {
-  f4v v;
+template <int V>
+struct Few<float, V, true> {
+  __attribute__((ext_vector_type(V))) float v;
 };
-template <>
-struct Four<__bf16, true> {
-  u2v v;
+template <int V>
+struct Few<__bf16, V, true> {
+  __attribute__((ext_vector_type(V / 2))) uint32_t v;
 };
-template <typename T, bool VEC>
-__device__ __forceinline__ void fetch_four(const T* p, int n, Four<T, VEC>& f) {
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void fetch_few(const T* p, int n, Few<T, V, VEC>& f) {
   if constexpr (VEC) {
     f.v = {};
     if (n > 0) f.v = *reinterpret_cast<const decltype(f.v)*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.v[i] = i < n ? p[i] : (T)0.0f;
+    for (int i = 0; i < V; ++i) f.v[i] = i < n ? p[i] : (T)0.0f;
   }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ float at_four(const Four<T, VEC>& f, int i) {
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ float at_few(const Few<T, V, VEC>& f, int i) {
   if constexpr (VEC && sizeof(T) == 2)
     return i & 1 ? bf16_hi(f.v[i / 2]) : bf16_lo(f.v[i / 2]);
   else
     return (float)f.v[i];
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void load_four(const T* p, int n, float (&v)[4]) {
-  Four<T, VEC> f;
-  fetch_four(p, n, f);
+template <bool VEC, int V, typename T>
+__device__ __forceinline__ void load_few(const T* p, int n, float (&v)[V]) {
+  Few<T, V, VEC> f;
+  fetch_few(p, n, f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = at_four(f, i);
+  for (int i = 0; i < V; ++i) v[i] = at_few(f, i);
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void store_four(T* p, int n, const float (&v)[4]) {
+template <bool VEC, int V, typename T>
+__device__ __forceinline__ void store_few(T* p, int n, const float (&v)[V]) {
   if constexpr (VEC) {
-    if (n > 0) store_vec<4>(p, v);
+    if (n <= 0) return;
+    Few<T, V, true> f;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (sizeof(T) == 2)
+        f.v[i / 2] = bf16_pair(v[i], v[i + 1]);
+      else
+        f.v[i] = v[i], f.v[i + 1] = v[i + 1];
+    }
+    *reinterpret_cast<decltype(f.v)*>(p) = f.v;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < n) store1(p + i, v[i]);
   }
 }
 
-// Four tokens of B and C for one token and four states a thread.
+// B and C into that layout, one token and two states a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(ScanArgs a, float* __restrict__ out) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int lp = a.ntiles * kScanTile, quads = a.np / 4;
-  const long long row = id / lp;  // (b G + g) quads + quad
-  if (row >= (long long)a.B * a.G * quads) return;
-  const int t = (int)(id - row * lp), w = (int)(row % quads), n = w * 4;
-  const long long bg = row / quads;
+  const int lp = a.ntiles * kScanTile, pairs = a.np / 2;
+  const long long row = id / lp;  // (b G + g) pairs + pair
+  if (row >= (long long)a.B * a.G * pairs) return;
+  const int t = (int)(id - row * lp), n = (int)(row % pairs) * 2;
+  const long long bg = row / pairs;
   const int b = (int)(bg / a.G), g = (int)(bg - (long long)b * a.G);
-  f4v bv = {0.0f, 0.0f, 0.0f, 0.0f}, cv = bv;
+  float2 bv = {0.0f, 0.0f}, cv = bv;
   if (t < scan_length(a, b)) {
     const T* bp = static_cast<const T*>(a.bm) + b * a.b_batch + t * a.b_row + (long long)g * a.b_group + n;
     const T* cp = static_cast<const T*>(a.cm) + b * a.c_batch + t * a.c_row + (long long)g * a.c_group + n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) bv[i] = load1(bp + i), cv[i] = load1(cp + i);
+    if (n < a.N) bv.x = load1(bp), cv.x = load1(cp);
+    if (n + 1 < a.N) bv.y = load1(bp + 1), cv.y = load1(cp + 1);
   }
-  f4v* o = reinterpret_cast<f4v*>(out + id * 8);
-  o[0] = bv, o[1] = cv;
+  float2* o = reinterpret_cast<float2*>(out) + row * lp * 2 + t / kScanGroup * 2 * kScanGroup + t % kScanGroup;
+  o[0] = bv;
+  o[kScanGroup] = cv;
 }
 
 // Where a workgroup works: blocks of channels are fastest, then the chunks of
@@ -175,7 +195,7 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t id) 
   return p;
 }
 
-// Rounds of 16 states over a tile; a lane's four states of one in memory: of
+// Rounds of 16 states over a tile; a lane's two states of one in memory: of
 // [.., H, N] as the caller has them, and of [.., np, H], coalesced, where the
 // kernels keep states for themselves.
 template <bool MANY>
@@ -183,71 +203,71 @@ __device__ __forceinline__ int scan_rounds(const ScanArgs& a) {
   return MANY ? a.np / 16 : 1;
 }
 __device__ __forceinline__ void load_states(const float* p, bool mine, const ScanArgs& a,
-                                            long long row, int r, int wave, float (&v)[4]) {
+                                            long long row, int r, int wave, float (&v)[kScanStates]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = (r * kScanWaves + wave) * 4 + i;
+  for (int i = 0; i < kScanStates; ++i) {
+    const int n = (r * kScanWaves + wave) * kScanStates + i;
     v[i] = p && mine && n < a.N ? p[row * a.N + n] : 0.0f;
   }
 }
 __device__ __forceinline__ void store_states(float* p, bool mine, const ScanArgs& a, long long row,
-                                             int r, int wave, const float (&v)[4]) {
+                                             int r, int wave, const float (&v)[kScanStates]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = (r * kScanWaves + wave) * 4 + i;
+  for (int i = 0; i < kScanStates; ++i) {
+    const int n = (r * kScanWaves + wave) * kScanStates + i;
     if (p && mine && n < a.N) p[row * a.N + n] = v[i];
   }
 }
 __device__ __forceinline__ long long state_at(const ScanArgs& a, long long row, int r, int wave, int h) {
-  return (row * a.np + (r * kScanWaves + wave) * 4) * a.H + h;
+  return (row * a.np + (r * kScanWaves + wave) * kScanStates) * a.H + h;
 }
 // Rows of A times log2 e, for exp2.
 __device__ __forceinline__ void load_rates(const ScanArgs& a, bool mine, int h, int r, int wave,
-                                           float (&v)[4]) {
+                                           float (&v)[kScanStates]) {
   load_states(a.a, mine, a, h, r, wave, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] *= kLog2E;
+  for (int i = 0; i < kScanStates; ++i) v[i] *= kLog2E;
 }
 
-// Four values a lane of each round: in registers for one, in LDS for more.
+// Two values a lane of each round: in registers for one, in LDS for more.
 constexpr int kScanRounds = kScanMaxN / 16;
 template <bool MANY>
 struct Rounds;
 template <>
 struct Rounds<false> {
   struct Lds {};
-  float v[4];
+  float v[kScanStates];
   __device__ __forceinline__ Rounds(Lds&) {}
-  __device__ __forceinline__ void get(int, float (&o)[4]) const {
+  __device__ __forceinline__ void get(int, float (&o)[kScanStates]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = v[i];
+    for (int i = 0; i < kScanStates; ++i) o[i] = v[i];
   }
-  __device__ __forceinline__ void set(int, const float (&o)[4]) {
+  __device__ __forceinline__ void set(int, const float (&o)[kScanStates]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = o[i];
+    for (int i = 0; i < kScanStates; ++i) v[i] = o[i];
   }
 };
 template <>
 struct Rounds<true> {
   struct Lds {
-    float v[kScanRounds][4][kScanThreads];
+    float v[kScanRounds][kScanStates][kScanThreads];
   };
   Lds& lds;
   __device__ __forceinline__ Rounds(Lds& l) : lds(l) {}
-  __device__ __forceinline__ void get(int r, float (&o)[4]) const {
+  __device__ __forceinline__ void get(int r, float (&o)[kScanStates]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = lds.v[r][i][threadIdx.x];
+    for (int i = 0; i < kScanStates; ++i) o[i] = lds.v[r][i][threadIdx.x];
   }
-  __device__ __forceinline__ void set(int r, const float (&o)[4]) {
+  __device__ __forceinline__ void set(int r, const float (&o)[kScanStates]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds.v[r][i][threadIdx.x] = o[i];
+    for (int i = 0; i < kScanStates; ++i) lds.v[r][i][threadIdx.x] = o[i];
   }
 };
 
 // s of a round through the chunks [from, to), upwards or downwards.
 __device__ __forceinline__ void join_chunks(const ScanArgs& a, const float* states, const float* steps,
                                             int b, int from, int to, int r, int wave, int h,
-                                            const float (&a2)[4], float (&s)[4]) {
+                                            const float (&a2)[kScanStates], float (&s)[kScanStates]) {
   const int way = from < to ? 1 : -1;
 #pragma unroll 4
   for (int c = from; c != to; c += way) {
@@ -255,7 +275,7 @@ __device__ __forceinline__ void join_chunks(const ScanArgs& a, const float* stat
     const float d = steps[row * a.H + h];
     const float* p = states + state_at(a, row, r, wave, h);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kScanStates; ++i)
       s[i] = fmaf(__builtin_amdgcn_exp2f(d * a2[i]), s[i], p[(long long)i * a.H]);
   }
 }
@@ -290,53 +310,53 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
   const bool mine = lane < p.nh;
   const int h = p.h0 + lane;
   Rounds<MANY> states(hold);
-  float a2[4], steps = 0.0f;
-  const float zero[4] = {};
+  float a2[kScanStates], steps = 0.0f;
+  const float zero[kScanStates] = {};
   for (int r = 0; r < rounds; ++r) states.set(r, zero);
   load_rates(a, mine, h, 0, wave, a2);
 
-  const int row = tid >> 4, c0 = (tid & 15) * 4, cn = p.nh - c0;
+  const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
   const T* xp = REV ? static_cast<const T*>(f.gy) + (long long)p.b * a.L * a.H
                     : static_cast<const T*>(a.x) + (long long)p.b * a.x_batch;
   const long long xrow = REV ? a.H : a.x_row;
   xp += p.h0 + c0;
   const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
-  float bias[4];
+  float bias[kScanCols];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
-  Four<T, VEC> xv, dv;
+  for (int i = 0; i < kScanCols; ++i) bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
+  Few<T, kScanCols, VEC> xv, dv;
   auto fetch = [&](int tile) {
     const int t = tile * kScanTile + row;
     const int n = t < len ? cn : 0;
-    fetch_four(xp + (n > 0 ? t * xrow : 0), n, xv);
-    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    fetch_few(xp + (n > 0 ? t * xrow : 0), n, xv);
+    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
   };
   auto put = [&](int tile) {
     const bool in = tile * kScanTile + row < len;
-    float d[4], g;
+    float d[kScanCols], g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i];
+    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[i];
     if (a.softplus) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &g);
+      for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &g);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = at_four(xv, i);
+    for (int i = 0; i < kScanCols; ++i) {
+      const float x = at_few(xv, i);
       du[tile & 1][row][c0 + i] = in ? make_float2(d[i], REV ? x : d[i] * x) : make_float2(0.0f, 0.0f);
     }
   };
   const int tiles = (len + kScanTile - 1) / kScanTile;
   const int last = p.last < tiles ? p.last : tiles, n = last - p.first;
   auto at = [&](int k) { return REV ? last - 1 - k : p.first + k; };
-  const size_t quad = (size_t)a.ntiles * kScanTile * 8;  // floats of four states
-  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
-  auto group_at = [&](int tile, int r, int g) {
-    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + (REV ? kGroups - 1 - g : g)) * kScanGroup * 8;
+  const size_t pair = (size_t)a.ntiles * kScanTile * 4;  // floats of two states
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
+  auto group_at = [&](int tile, int r, int g) {  // B, or C for REV
+    return bc + r * kScanWaves * pair + (((size_t)tile * kGroups + (REV ? kGroups - 1 - g : g)) * 2 + REV) * kScanGroup * 2;
   };
-  BcGroup next = {};
+  u16s next = {};
   if (n > 0) {
-    next = load_group(group_at(at(0), 0, 0));
+    next = load_uniform(group_at(at(0), 0, 0));
     fetch(at(0));
     put(at(0));
     if (n > 1) fetch(at(1));
@@ -349,34 +369,35 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) q[t] = du[tile & 1][t][lane];
     for (int r = 0; r < rounds; ++r) {
-      float s[4], a3[4];
+      float s[kScanStates], a3[kScanStates];
       states.get(r, s);
       if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         wait_groups();
-        const BcGroup now = next;
+        const u16s now = next;
         if (g + 1 < kGroups)
-          next = load_group(group_at(tile, r, g + 1));
+          next = load_uniform(group_at(tile, r, g + 1));
         else  // of the next round or tile; the last one's own again
-          next = load_group(r + 1 < rounds ? group_at(tile, r + 1, 0) : group_at(at(k + 1 < n ? k + 1 : k), 0, 0));
+          next = load_uniform(r + 1 < rounds ? group_at(tile, r + 1, 0) : group_at(at(k + 1 < n ? k + 1 : k), 0, 0));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int jj = 0; jj < kScanGroup; ++jj) {
           const int j = REV ? kScanGroup - 1 - jj : jj;
           const int t = (REV ? kGroups - 1 - g : g) * kScanGroup + j;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kScanStates; ++i) {
             const float e = __builtin_amdgcn_exp2f(q[t].x * a2[i]);
-            s[i] = REV ? e * fmaf(now.c(j, i), q[t].y, s[i]) : fmaf(e, s[i], q[t].y * now.b(j, i));
+            s[i] = REV ? e * fmaf(uniform_at(now, j, i), q[t].y, s[i]) : fmaf(e, s[i], q[t].y * uniform_at(now, j, i));
           }
         }
+        pin(s);
         __builtin_amdgcn_sched_barrier(0);
       }
       states.set(r, s);
       if (MANY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
+        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
       }
     }
     float sum = 0.0f;
@@ -392,10 +413,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
   if (!mine) return;
   const long long out = (long long)p.b * a.chunks + p.c;
   for (int r = 0; r < rounds; ++r) {
-    float s[4];
+    float s[kScanStates];
     states.get(r, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.states[state_at(a, out, r, wave, h) + (long long)i * a.H] = s[i];
+    for (int i = 0; i < kScanStates; ++i) f.states[state_at(a, out, r, wave, h) + (long long)i * a.H] = s[i];
   }
   if (wave == 0) f.steps[out * a.H + h] = steps;
 }
@@ -423,53 +444,53 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   const int h = p.h0 + lane;
 
   Rounds<MANY> states(hold);
-  float a2[4];
+  float a2[kScanStates];
   for (int r = rounds - 1; r >= 0; --r) {
-    float s[4];
+    float s[kScanStates];
     load_rates(a, mine, h, r, wave, a2);
     load_states(a.state, mine, a, (long long)p.b * a.H + h, r, wave, s);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, 0, p.c, r, wave, h, a2, s);
     states.set(r, s);
   }
 
-  // Loading and storing: token tid / 16 of a tile, four channels.
-  const int row = tid >> 4, c0 = (tid & 15) * 4, cn = p.nh - c0;
+  // Loading and storing: token tid / 32 of a tile, two channels.
+  const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
   const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
   const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
   T* yo = static_cast<T*>(f.y) + (long long)p.b * a.L * a.H + p.h0 + c0;
-  float bias[4], dskip[4], xk[4];
+  float bias[kScanCols], dskip[kScanCols], xk[kScanCols];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kScanCols; ++i) {
     bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
     dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
   }
-  Four<T, VEC> xv, dv;
+  Few<T, kScanCols, VEC> xv, dv;
   auto fetch = [&](int tile) {
     const int t = tile * kScanTile + row;
     const int n = t < len ? cn : 0;
-    fetch_four(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    fetch_few(xp + (n > 0 ? t * a.x_row : 0), n, xv);
+    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
   };
   auto put = [&](int tile) {
     const bool in = tile * kScanTile + row < len;
-    float d[4], g;
+    float d[kScanCols], g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i], xk[i] = at_four(xv, i);
+    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[i], xk[i] = at_few(xv, i);
     if (a.softplus) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &g);
+      for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &g);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kScanCols; ++i)
       du[tile & 1][row][c0 + i] = in ? make_float2(d[i], d[i] * xk[i]) : make_float2(0.0f, 0.0f);
   };
 
   const int tiles = (len + kScanTile - 1) / kScanTile;
   const int last = p.last < tiles ? p.last : tiles;
-  const size_t quad = (size_t)a.ntiles * kScanTile * 8;  // floats of four states
-  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
+  const size_t pair = (size_t)a.ntiles * kScanTile * 4;  // floats of two states
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
   auto group_at = [&](int tile, int r, int g) {
-    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + g) * kScanGroup * 8;
+    return bc + r * kScanWaves * pair + ((size_t)tile * kGroups + g) * kScanGroup * 4;
   };
   BcGroup next = {};
   if (p.first < last) {
@@ -487,13 +508,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) q[t] = du[buf][t][lane], y[t] = 0.0f;
     for (int r = 0; r < rounds; ++r) {
-      float s[4], a3[4];
+      float s[kScanStates], a3[kScanStates];
       states.get(r, s);
       if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
       if (f.saved && mine) {
         float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sp[(long long)i * a.H] = s[i];
+        for (int i = 0; i < kScanStates; ++i) sp[(long long)i * a.H] = s[i];
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
@@ -509,24 +530,25 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
         for (int j = 0; j < kScanGroup; ++j) {
           const int t = g * kScanGroup + j;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kScanStates; ++i) {
             s[i] = fmaf(__builtin_amdgcn_exp2f(q[t].x * a2[i]), s[i], q[t].y * now.b(j, i));
             y[t] = fmaf(now.c(j, i), s[i], y[t]);
           }
         }
+        pin(s);
         __builtin_amdgcn_sched_barrier(0);
       }
       states.set(r, s);
       if (MANY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
+        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
       }
     }
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) yp[buf][wave][t][lane] = y[t];
-    float xr[4];
+    float xr[kScanCols];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xr[i] = xk[i];
+    for (int i = 0; i < kScanCols; ++i) xr[i] = xk[i];
     if (tile + 1 < last) {
       put(tile + 1);
       if (tile + 2 < last) fetch(tile + 2);
@@ -534,23 +556,23 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
     __syncthreads();
     const int t = tile * kScanTile + row;
     if (t < a.L) {
-      float out[4];
+      float out[kScanCols];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kScanCols; ++i) {
         float v = dskip[i] * xr[i];
 #pragma unroll
         for (int w = 0; w < kScanWaves; ++w) v += yp[buf][w][row][c0 + i];
         out[i] = t < len ? v : 0.0f;
       }
-      store_four<VEC>(yo + (long long)t * a.H, cn, out);
+      store_few<VEC, kScanCols>(yo + (long long)t * a.H, cn, out);
     }
   }
-  const float zero[4] = {};
+  const float zero[2] = {};
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile)
-    if (tile * kScanTile + row < a.L) store_four<VEC>(yo + (long long)(tile * kScanTile + row) * a.H, cn, zero);
+    if (tile * kScanTile + row < a.L) store_few<VEC, kScanCols>(yo + (long long)(tile * kScanTile + row) * a.H, cn, zero);
   if (p.c < a.chunks - 1) return;
   for (int r = 0; r < rounds; ++r) {
-    float s[4];
+    float s[kScanStates];
     states.get(r, s);
     store_states(f.state_out, mine, a, (long long)p.b * a.H + h, r, wave, s);
   }
@@ -566,7 +588,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 // all 16 tokens in registers, then backward. Sums over the states go through
 // LDS as y does; sums over the channels are butterflies over the lanes that
 // halve the number of values at each level and leave one (token, state) in
-// each lane: 126 folds for the 128 values of a wave's round.
+// each lane: 63 folds for the 64 values of a wave's round.
 // ---------------------------------------------------------------------------
 struct ScanBwdArgs {
   ScanArgs s;
@@ -617,15 +639,15 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   const int last = p.last < tiles ? p.last : tiles;
 
   Rounds<MANY> qs(hold_q), gas(hold_a);
-  const float zero[4] = {};
-  float a2[4], s0[4];  // of the round at hand
-  auto load_saved = [&](int tile, int r, float(&v)[4]) {
+  const float zero[2] = {};
+  float a2[kScanStates], s0[kScanStates];  // of the round at hand
+  auto load_saved = [&](int tile, int r, float(&v)[kScanStates]) {
     const float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = mine ? sp[(long long)i * a.H] : 0.0f;
+    for (int i = 0; i < kScanStates; ++i) v[i] = mine ? sp[(long long)i * a.H] : 0.0f;
   };
   for (int r = rounds - 1; r >= 0; --r) {
-    float q[4];
+    float q[kScanStates];
     load_rates(a, mine, h, r, wave, a2);
     load_states(f.gstate_out, mine, a, (long long)p.b * a.H + h, r, wave, q);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, a.chunks - 1, p.c, r, wave, h, a2, q);
@@ -633,41 +655,42 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
     gas.set(r, zero);
   }
 
-  const int row = tid >> 4, c0 = (tid & 15) * 4, cn = p.nh - c0;
+  const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
   const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
   const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
   const long long yb = (long long)p.b * a.L * a.H + p.h0 + c0;
   const T* gp = static_cast<const T*>(f.gy) + yb;
   T* gxp = static_cast<T*>(f.gx) + yb;
   T* gdp = static_cast<T*>(f.gdt) + yb;
-  float bias[4], dskip[4], gd[4] = {}, gbias[4] = {};
+  float bias[kScanCols], dskip[kScanCols], gd[kScanCols] = {}, gbias[kScanCols] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kScanCols; ++i) {
     bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
     dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
   }
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile) {
     const int t = tile * kScanTile + row;
     if (t >= a.L) continue;
-    store_four<VEC>(gxp + (long long)t * a.H, cn, zero);
-    store_four<VEC>(gdp + (long long)t * a.H, cn, zero);
+    store_few<VEC, kScanCols>(gxp + (long long)t * a.H, cn, zero);
+    store_few<VEC, kScanCols>(gdp + (long long)t * a.H, cn, zero);
   }
-  Four<T, VEC> xv, dv, gv;
+  Few<T, kScanCols, VEC> xv, dv, gv;
   auto fetch = [&](int tile) {
     const int t = tile * kScanTile + row;
     const int n = t < len ? cn : 0;
-    fetch_four(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    fetch_four(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
-    fetch_four(gp + (n > 0 ? (long long)t * a.H : 0), n, gv);
+    fetch_few(xp + (n > 0 ? t * a.x_row : 0), n, xv);
+    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    fetch_few(gp + (n > 0 ? (long long)t * a.H : 0), n, gv);
   };
-  const size_t quad = (size_t)a.ntiles * kScanTile * 8;
-  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 4) + wave) * quad;
+  const size_t pair = (size_t)a.ntiles * kScanTile * 4;
+  const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
   auto group_at = [&](int tile, int r, int g) {
-    return bc + r * kScanWaves * quad + ((size_t)tile * kGroups + g) * kScanGroup * 8;
+    return bc + r * kScanWaves * pair + ((size_t)tile * kGroups + g) * kScanGroup * 4;
   };
-  BcGroup next = {};
+  BcGroup next;
+  u16s nextb = {};
   if (p.first < last) {
-    next = load_group(group_at(last - 1, 0, 0));
+    nextb = load_uniform(group_at(last - 1, 0, 0));
     fetch(last - 1);
     load_saved(last - 1, 0, s0);
   }
@@ -675,51 +698,55 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   for (int tile = last - 1; tile >= p.first; --tile) {
     const int t0 = tile * kScanTile;
     const bool in = t0 + row < len;  // tokens past the end change nothing
-    float d[4], sg[4];
-    Four<T, VEC> xk = xv, gk = gv;
+    float d[kScanCols], sg[kScanCols];
+    Few<T, kScanCols, VEC> xk = xv, gk = gv;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = at_four(dv, i) + bias[i], sg[i] = 1.0f;
+    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[i], sg[i] = 1.0f;
     if (a.softplus) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = softplus_f32(d[i], &sg[i]);
+      for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &sg[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      du[row][c0 + i] = in ? make_float2(d[i], d[i] * at_four(xk, i)) : make_float2(0.0f, 0.0f);
-      gys[row][c0 + i] = in ? at_four(gk, i) : 0.0f;
+    for (int i = 0; i < kScanCols; ++i) {
+      du[row][c0 + i] = in ? make_float2(d[i], d[i] * at_few(xk, i)) : make_float2(0.0f, 0.0f);
+      gys[row][c0 + i] = in ? at_few(gk, i) : 0.0f;
     }
     if (tile > p.first) fetch(tile - 1);
     __syncthreads();
     for (int r = 0; r < rounds; ++r) {
-      float s[kScanTile + 1][4], e[kScanTile][4], q[4], a3[4];
+      float s[kScanTile + 1][kScanStates], e[kScanTile][kScanStates], q[kScanStates], a3[kScanStates];
       const bool more = r + 1 < rounds;
       const int tile2 = more ? tile : tile > p.first ? tile - 1 : tile, r2 = more ? r + 1 : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[0][i] = s0[i];
+      for (int i = 0; i < kScanStates; ++i) s[0][i] = s0[i];
       load_saved(tile2, r2, s0);
       if (MANY) load_rates(a, mine, h, r2, wave, a3);
+      // Forward with B alone, then back with both: the last group is first.
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         float2 w[kScanGroup];
 #pragma unroll
         for (int j = 0; j < kScanGroup; ++j) w[j] = du[g * kScanGroup + j][lane];
         wait_groups();
-        const BcGroup now = next;
-        // the last group is also the first one on the way back
-        if (g + 1 < kGroups) next = load_group(group_at(tile, r, g + 1));
+        const u16s now = nextb;
+        if (g + 1 < kGroups)
+          nextb = load_uniform(group_at(tile, r, g + 1));
+        else
+          next = load_group(group_at(tile, r, g));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kScanGroup; ++j) {
           const int t = g * kScanGroup + j;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kScanStates; ++i) {
             e[t][i] = __builtin_amdgcn_exp2f(w[j].x * a2[i]);
-            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * now.b(j, i));
+            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(now, j, i));
           }
         }
+        pin(s[(g + 1) * kScanGroup]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      float rb[kScanTile], rc[kScanTile], ga[4] = {};
+      float rb[kScanTile], rc[kScanTile], ga[kScanStates] = {};
       qs.get(r, q);
 #pragma unroll
       for (int g = kGroups - 1; g >= 0; --g) {
@@ -734,14 +761,17 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
         }
         wait_groups();
         const BcGroup now = next;
-        next = load_group(g > 0 ? group_at(tile, r, g - 1) : group_at(tile2, r2, 0));
+        if (g > 0)
+          next = load_group(group_at(tile, r, g - 1));
+        else
+          nextb = load_uniform(group_at(tile2, r2, 0));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = kScanGroup - 1; j >= 0; --j) {
           const int t = g * kScanGroup + j;
-          float vb[4], vc[4];
+          float vb[kScanStates], vc[kScanStates];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kScanStates; ++i) {
             const float G = fmaf(now.c(j, i), gyt[j], q[i]);
             o1[j] = fmaf(now.b(j, i), G, o1[j]);
             vb[i] = G * w[j].y;
@@ -751,80 +781,79 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
             o2[j] = fmaf(k, a2[i], o2[j]);
             ga[i] = fmaf(k, w[j].x, ga[i]);
           }
-          rb[t] = fold16(fold32(vb[0], vb[2]), fold32(vb[1], vb[3]));
-          rc[t] = fold16(fold32(vc[0], vc[2]), fold32(vc[1], vc[3]));
+          rb[t] = fold32(vb[0], vb[1]);
+          rc[t] = fold32(vc[0], vc[1]);
           p1[wave][t][lane] = o1[j];
           p2[wave][t][lane] = o2[j];
           if (t < 8) {
-            rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 8], lane & 8);
-            rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 8], lane & 8);
+            rb[t] = fold16(rb[t], rb[t + 8]);
+            rc[t] = fold16(rc[t], rc[t + 8]);
           }
           if (t < 4) {
-            rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 4], lane & 4);
-            rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 4], lane & 4);
+            rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 4], lane & 8);
+            rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 4], lane & 8);
           }
         }
+        pin(q);
         __builtin_amdgcn_sched_barrier(0);
       }
       qs.set(r, q);
       gas.get(r, q);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ga[i] += q[i];
+      for (int i = 0; i < kScanStates; ++i) ga[i] += q[i];
       gas.set(r, ga);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        rb[t] = fold_row<kDppXor2>(rb[t], rb[t + 2], lane & 2);
-        rc[t] = fold_row<kDppXor2>(rc[t], rc[t + 2], lane & 2);
+        rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 2], lane & 4);
+        rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 2], lane & 4);
       }
-      rb[0] = fold_row<kDppXor1>(rb[0], rb[1], lane & 1);
-      rc[0] = fold_row<kDppXor1>(rc[0], rc[1], lane & 1);
-      // lane: token lane % 16, state lane / 16
-      const int t = t0 + (lane & 15);
-      if (t < len) {
-        float* o = f.part_bc + (((long long)p.blk * a.B + p.b) * a.L + t) * 2 * a.np +
-                   (r * kScanWaves + wave) * 4 + (lane >> 4);
-        o[0] = rb[0];
-        o[a.np] = rc[0];
-      }
+      rb[0] = fold_row<kDppXor2>(rb[0], rb[1], lane & 2);
+      rc[0] = fold_row<kDppXor2>(rc[0], rc[1], lane & 2);
+      rb[0] = fold_row<kDppXor1>(rb[0], rc[0], lane & 1);
+      // lane: state lane / 32, token lane / 2 % 16, B or C
+      const int t = t0 + (lane >> 1 & 15);
+      if (t < len)
+        f.part_bc[((((long long)p.blk * a.B + p.b) * a.L + t) * 2 + (lane & 1)) * a.np +
+                  (r * kScanWaves + wave) * kScanStates + (lane >> 5)] = rb[0];
       if (MANY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a2[i] = a3[i];
+        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
       }
     }
     __syncthreads();
     const int t = t0 + row;
     if (t < a.L) {
-      float ox[4], od[4];
+      float ox[kScanCols], od[kScanCols];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kScanCols; ++i) {
         float g1 = 0.0f, g2 = 0.0f;
 #pragma unroll
         for (int w = 0; w < kScanWaves; ++w) g1 += p1[w][row][c0 + i], g2 += p2[w][row][c0 + i];
-        const float x = at_four(xk, i), gy = at_four(gk, i);  // 0 past the end
+        const float x = at_few(xk, i), gy = at_few(gk, i);  // 0 past the end
         ox[i] = in ? fmaf(d[i], g1, dskip[i] * gy) : 0.0f;
         od[i] = in ? fmaf(x, g1, kLn2 * g2) * sg[i] : 0.0f;
         gd[i] = fmaf(gy, x, gd[i]);
         gbias[i] += od[i];
       }
-      store_four<VEC>(gxp + (long long)t * a.H, cn, ox);
-      store_four<VEC>(gdp + (long long)t * a.H, cn, od);
+      store_few<VEC, kScanCols>(gxp + (long long)t * a.H, cn, ox);
+      store_few<VEC, kScanCols>(gdp + (long long)t * a.H, cn, od);
     }
     __syncthreads();
   }
   const long long part = (long long)p.b * a.chunks + p.c;
   for (int r = 0; r < rounds; ++r) {
-    float v[4];
+    float v[kScanStates];
     gas.get(r, v);
     if (mine) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f.part_a[state_at(a, part, r, wave, h) + (long long)i * a.H] = v[i];
+      for (int i = 0; i < kScanStates; ++i) f.part_a[state_at(a, part, r, wave, h) + (long long)i * a.H] = v[i];
     }
     qs.get(r, v);
     if (p.c == 0) store_states(f.gstate, mine, a, (long long)p.b * a.H + h, r, wave, v);
   }
   // The sums over the tokens of a tile's rows.
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p1[0][row][c0 + i] = gd[i], p2[0][row][c0 + i] = gbias[i];
+  for (int i = 0; i < kScanCols; ++i) p1[0][row][c0 + i] = gd[i], p2[0][row][c0 + i] = gbias[i];
   __syncthreads();
   if (tid < 2 * kScanCh && mine) {
     float v = 0.0f;
@@ -881,16 +910,16 @@ __global__ __launch_bounds__(256) void scan_step_kernel(
   const T* bp = bm + b * b_row + (long long)g * b_group + n0;
   const T* cp = cm + b * c_row + (long long)g * c_group + n0;
   float s[4], av[4], bv[4], cv[4], out = 0.0f;
-  load_four<VEC>(sp, N - n0, s);
-  load_four<VEC>(ap, N - n0, av);
-  load_four<VEC>(bp, N - n0, bv);
-  load_four<VEC>(cp, N - n0, cv);
+  load_few<VEC>(sp, N - n0, s);
+  load_few<VEC>(ap, N - n0, av);
+  load_few<VEC>(bp, N - n0, bv);
+  load_few<VEC>(cp, N - n0, cv);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     s[i] = fmaf(__builtin_amdgcn_exp2f(d * (av[i] * kLog2E)), s[i], d * xv * bv[i]);
     out = fmaf(cv[i], s[i], out);
   }
-  store_four<VEC>(sp, N - n0, s);
+  store_few<VEC>(sp, N - n0, s);
 #pragma unroll
   for (int k = 1; k < PER; k *= 2) out += __shfl_xor(out, k);
   if (n0 == 0) store1(y + (long long)b * H + h, fmaf(dskip ? dskip[h] : 0.0f, xv, out));
