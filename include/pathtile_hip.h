@@ -438,7 +438,7 @@ int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* 
  *   y[b,t,h] = sum_n C[b,t,g,n] s[n] + D[h] x[b,t,h]
  * x, dt [B, L, H]; B, C [B, L, G, N] with contiguous states (b_group: between
  * groups); A [H, N]; D and dt_bias [H] or NULL (0); the first state [B, H, N]
- * or NULL (0). delta must not be negative with A positive beyond FP32's range.
+ * or NULL (0). H and the row strides of x and dt are below 2^25.
  * _sizes gives the bytes of the workspaces and of `saved`, which _fwd fills
  * where not NULL (the state before every 16 tokens) and _bwd takes with the
  * same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;

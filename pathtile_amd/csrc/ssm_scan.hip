@@ -42,6 +42,9 @@ static int check_scan(const pt_scan_inputs* in, int L) {
     return PT_ERR_SHAPE;
   if (in->b_group < 0 || in->c_group < 0 || in->b_group >= (1LL << 31) || in->c_group >= (1LL << 31))
     return PT_ERR_SHAPE;
+  for (long long row : {in->x_row, in->dt_row})
+    if (L > 1 && (row < 0 || row >= kScanMaxRow)) return PT_ERR_SHAPE;
+  if (in->H >= kScanMaxRow) return PT_ERR_SHAPE;
   if (in->B == 0) return PT_OK;
   return in->x && in->dt && in->a && in->b && in->c ? PT_OK : PT_ERR_NULL;
 }

@@ -66,21 +66,35 @@ __device__ __forceinline__ float softplus_f32(float v, float* grad) {
 // B and C as the waves read them: for every two states and eight tokens 16
 // floats B[8][2] and 16 of C that all lanes share, in scalar registers.
 // [B, G, np / 2, 2 ntiles, 2, 8, 2]; zeros from state N on and past a
-// sequence's end, so that a tile is always whole.
-constexpr int kScanGroup = 8;  // tokens of a scalar load
+// sequence's end, so that a tile is always whole. A load is of one of both or
+// of both for eight tokens, or, where the addresses need the room, of both for
+// four.
+constexpr int kScanGroup = 8, kScanHalf = 4;
 typedef uint32_t u16s __attribute__((ext_vector_type(16)));
-typedef const __attribute__((address_space(4))) u16s* scalar_ptr;
-__device__ __forceinline__ u16s load_uniform(const float* p) { return *(scalar_ptr)(uintptr_t)p; }
-__device__ __forceinline__ float uniform_at(const u16s& q, int t, int i) {
+typedef uint32_t u8s __attribute__((ext_vector_type(8)));
+template <typename V>
+__device__ __forceinline__ V load_uniform(const float* p) {
+  return *(const __attribute__((address_space(4))) V*)(uintptr_t)p;
+}
+template <typename V>
+__device__ __forceinline__ float uniform_at(const V& q, int t, int i) {
   return __uint_as_float(q[t * 2 + i]);
 }
-struct BcGroup {
-  u16s bq, cq;
+template <typename V>
+struct BcOf {
+  V bq, cq;
   __device__ __forceinline__ float b(int t, int i) const { return uniform_at(bq, t, i); }
   __device__ __forceinline__ float c(int t, int i) const { return uniform_at(cq, t, i); }
 };
+using BcGroup = BcOf<u16s>;
+using BcHalf = BcOf<u8s>;
 __device__ __forceinline__ BcGroup load_group(const float* p) {
-  return {load_uniform(p), load_uniform(p + 16)};
+  return {load_uniform<u16s>(p), load_uniform<u16s>(p + 2 * kScanGroup)};
+}
+// tokens 4 k .. 4 k + 3 of the tile at `p`
+__device__ __forceinline__ BcHalf load_half(const float* p, int k) {
+  p += (k >> 1) * 4 * kScanGroup + (k & 1) * 2 * kScanHalf;
+  return {load_uniform<u8s>(p), load_uniform<u8s>(p + 2 * kScanGroup)};
 }
 // Keeps what led to these values before what follows.
 template <int N>
@@ -92,7 +106,7 @@ __device__ __forceinline__ void pin(float (&v)[N]) {
 // a group comes before the next one is asked for, and the group in between is
 // worked on while that is under way.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
-__device__ __forceinline__ void wait_groups() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0)
+__device__ __forceinline__ void wait_scalars() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0)
 
 // V neighbouring values, those below `n` (0 elsewhere), as they are in memory
 // while they are under way.
@@ -151,6 +165,14 @@ __device__ __forceinline__ void store_few(T* p, int n, const float (&v)[V]) {
       if (i < n) store1(p + i, v[i]);
   }
 }
+
+// Addresses are a base that all lanes share, in scalar registers, and a lane's
+// offset in bytes, below 2^31 within a tile.
+template <typename T>
+__device__ __forceinline__ T* lane_at(T* base, uint32_t bytes) {
+  return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + bytes);
+}
+constexpr long long kScanMaxRow = 1LL << 25;  // values: 16 rows of FP32 are 2^31 bytes
 
 // B and C into that layout, one token and two states a thread.
 template <typename T>
@@ -316,20 +338,22 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
   load_rates(a, mine, h, 0, wave, a2);
 
   const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
+  const long long xrow = REV ? a.H : a.x_row;
   const T* xp = REV ? static_cast<const T*>(f.gy) + (long long)p.b * a.L * a.H
                     : static_cast<const T*>(a.x) + (long long)p.b * a.x_batch;
-  const long long xrow = REV ? a.H : a.x_row;
-  xp += p.h0 + c0;
-  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
+  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0;
+  xp += p.h0;
+  const uint32_t xo = (uint32_t)(row * xrow + c0) * sizeof(T), dto = (uint32_t)(row * a.dt_row + c0) * sizeof(T);
   float bias[kScanCols];
 #pragma unroll
   for (int i = 0; i < kScanCols; ++i) bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
   Few<T, kScanCols, VEC> xv, dv;
   auto fetch = [&](int tile) {
-    const int t = tile * kScanTile + row;
-    const int n = t < len ? cn : 0;
-    fetch_few(xp + (n > 0 ? t * xrow : 0), n, xv);
-    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    xv = {}, dv = {};
+    if (tile * kScanTile + row < len && cn > 0) {
+      fetch_few(lane_at(xp + (long long)tile * kScanTile * xrow, xo), cn, xv);
+      fetch_few(lane_at(dp + (long long)tile * kScanTile * a.dt_row, dto), cn, dv);
+    }
   };
   auto put = [&](int tile) {
     const bool in = tile * kScanTile + row < len;
@@ -342,8 +366,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
     }
 #pragma unroll
     for (int i = 0; i < kScanCols; ++i) {
-      const float x = at_few(xv, i);
-      du[tile & 1][row][c0 + i] = in ? make_float2(d[i], REV ? x : d[i] * x) : make_float2(0.0f, 0.0f);
+      const float x = at_few(xv, i), z = in ? d[i] : 0.0f;  // past the end nothing changes
+      du[tile & 1][row][c0 + i] = make_float2(z, REV ? x : z * x);
     }
   };
   const int tiles = (len + kScanTile - 1) / kScanTile;
@@ -356,7 +380,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
   };
   u16s next = {};
   if (n > 0) {
-    next = load_uniform(group_at(at(0), 0, 0));
+    next = load_uniform<u16s>(group_at(at(0), 0, 0));
     fetch(at(0));
     put(at(0));
     if (n > 1) fetch(at(1));
@@ -369,17 +393,18 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) q[t] = du[tile & 1][t][lane];
     for (int r = 0; r < rounds; ++r) {
+      const bool more = r + 1 < rounds;
       float s[kScanStates], a3[kScanStates];
       states.get(r, s);
-      if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
+      if (MANY) load_rates(a, mine, h, more ? r + 1 : 0, wave, a3);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        wait_groups();
+        wait_scalars();
         const u16s now = next;
         if (g + 1 < kGroups)
-          next = load_uniform(group_at(tile, r, g + 1));
+          next = load_uniform<u16s>(group_at(tile, r, g + 1));
         else  // of the next round or tile; the last one's own again
-          next = load_uniform(r + 1 < rounds ? group_at(tile, r + 1, 0) : group_at(at(k + 1 < n ? k + 1 : k), 0, 0));
+          next = load_uniform<u16s>(more ? group_at(tile, r + 1, 0) : group_at(at(k + 1 < n ? k + 1 : k), 0, 0));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int jj = 0; jj < kScanGroup; ++jj) {
@@ -388,7 +413,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
 #pragma unroll
           for (int i = 0; i < kScanStates; ++i) {
             const float e = __builtin_amdgcn_exp2f(q[t].x * a2[i]);
-            s[i] = REV ? e * fmaf(uniform_at(now, j, i), q[t].y, s[i]) : fmaf(e, s[i], q[t].y * uniform_at(now, j, i));
+            s[i] = REV ? e * fmaf(uniform_at(now, j, i), q[t].y, s[i])
+                       : fmaf(e, s[i], q[t].y * uniform_at(now, j, i));
           }
         }
         pin(s);
@@ -442,6 +468,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
   const int h = p.h0 + lane;
+  const uint32_t ho = (uint32_t)h * sizeof(float);
 
   Rounds<MANY> states(hold);
   float a2[kScanStates];
@@ -455,9 +482,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 
   // Loading and storing: token tid / 32 of a tile, two channels.
   const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
-  const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
-  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
-  T* yo = static_cast<T*>(f.y) + (long long)p.b * a.L * a.H + p.h0 + c0;
+  const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0;
+  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0;
+  T* op = static_cast<T*>(f.y) + (long long)p.b * a.L * a.H + p.h0;
+  const uint32_t xo = (uint32_t)(row * a.x_row + c0) * sizeof(T), dto = (uint32_t)(row * a.dt_row + c0) * sizeof(T);
+  const uint32_t oo = (uint32_t)(row * a.H + c0) * sizeof(T);
   float bias[kScanCols], dskip[kScanCols], xk[kScanCols];
 #pragma unroll
   for (int i = 0; i < kScanCols; ++i) {
@@ -466,10 +495,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   }
   Few<T, kScanCols, VEC> xv, dv;
   auto fetch = [&](int tile) {
-    const int t = tile * kScanTile + row;
-    const int n = t < len ? cn : 0;
-    fetch_few(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
+    xv = {}, dv = {};
+    if (tile * kScanTile + row < len && cn > 0) {
+      fetch_few(lane_at(xp + (long long)tile * kScanTile * a.x_row, xo), cn, xv);
+      fetch_few(lane_at(dp + (long long)tile * kScanTile * a.dt_row, dto), cn, dv);
+    }
   };
   auto put = [&](int tile) {
     const bool in = tile * kScanTile + row < len;
@@ -481,8 +511,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
       for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &g);
     }
 #pragma unroll
-    for (int i = 0; i < kScanCols; ++i)
-      du[tile & 1][row][c0 + i] = in ? make_float2(d[i], d[i] * xk[i]) : make_float2(0.0f, 0.0f);
+    for (int i = 0; i < kScanCols; ++i) {
+      const float z = in ? d[i] : 0.0f;  // past the end nothing changes
+      du[tile & 1][row][c0 + i] = make_float2(z, z * xk[i]);
+    }
   };
 
   const int tiles = (len + kScanTile - 1) / kScanTile;
@@ -508,23 +540,23 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) q[t] = du[buf][t][lane], y[t] = 0.0f;
     for (int r = 0; r < rounds; ++r) {
+      const bool more = r + 1 < rounds;
       float s[kScanStates], a3[kScanStates];
       states.get(r, s);
-      if (MANY) load_rates(a, mine, h, r + 1 < rounds ? r + 1 : 0, wave, a3);
+      if (MANY) load_rates(a, mine, h, more ? r + 1 : 0, wave, a3);
       if (f.saved && mine) {
-        float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
+        float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, 0);
 #pragma unroll
-        for (int i = 0; i < kScanStates; ++i) sp[(long long)i * a.H] = s[i];
+        for (int i = 0; i < kScanStates; ++i) *lane_at(sp + (long long)i * a.H, ho) = s[i];
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        wait_groups();
+        wait_scalars();
         const BcGroup now = next;
         if (g + 1 < kGroups)
           next = load_group(group_at(tile, r, g + 1));
         else  // of the next round or tile; the last one's own again
-          next = load_group(r + 1 < rounds ? group_at(tile, r + 1, 0)
-                                           : group_at(tile + 1 < last ? tile + 1 : tile, 0, 0));
+          next = load_group(more ? group_at(tile, r + 1, 0) : group_at(tile + 1 < last ? tile + 1 : tile, 0, 0));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kScanGroup; ++j) {
@@ -564,12 +596,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
         for (int w = 0; w < kScanWaves; ++w) v += yp[buf][w][row][c0 + i];
         out[i] = t < len ? v : 0.0f;
       }
-      store_few<VEC, kScanCols>(yo + (long long)t * a.H, cn, out);
+      store_few<VEC, kScanCols>(lane_at(op + (long long)tile * kScanTile * a.H, oo), cn, out);
     }
   }
-  const float zero[2] = {};
+  const float zero[kScanCols] = {};
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile)
-    if (tile * kScanTile + row < a.L) store_few<VEC, kScanCols>(yo + (long long)(tile * kScanTile + row) * a.H, cn, zero);
+    if (tile * kScanTile + row < a.L)
+      store_few<VEC, kScanCols>(lane_at(op + (long long)tile * kScanTile * a.H, oo), cn, zero);
   if (p.c < a.chunks - 1) return;
   for (int r = 0; r < rounds; ++r) {
     float s[kScanStates];
@@ -624,7 +657,7 @@ constexpr int kDppRor8 = 0x128, kDppHalfMirror = 0x141, kDppXor2 = 0x4e, kDppXor
 
 template <typename T, bool MANY, bool VEC>
 __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f) {
-  constexpr int kGroups = kScanTile / kScanGroup;
+  constexpr int kGroups = kScanTile / kScanGroup, kHalves = kScanTile / kScanHalf;
   __shared__ float2 du[kScanTile][kScanCh];
   __shared__ float gys[kScanTile][kScanCh];
   __shared__ float p1[kScanWaves][kScanTile][kScanCh], p2[kScanWaves][kScanTile][kScanCh];
@@ -635,16 +668,17 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
   const int h = p.h0 + lane;
+  const uint32_t ho = (uint32_t)h * sizeof(float);
   const int tiles = (len + kScanTile - 1) / kScanTile;
   const int last = p.last < tiles ? p.last : tiles;
 
   Rounds<MANY> qs(hold_q), gas(hold_a);
-  const float zero[2] = {};
+  const float zero[kScanStates] = {};
   float a2[kScanStates], s0[kScanStates];  // of the round at hand
   auto load_saved = [&](int tile, int r, float(&v)[kScanStates]) {
-    const float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, h);
+    const float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, 0);
 #pragma unroll
-    for (int i = 0; i < kScanStates; ++i) v[i] = mine ? sp[(long long)i * a.H] : 0.0f;
+    for (int i = 0; i < kScanStates; ++i) v[i] = mine ? *lane_at(sp + (long long)i * a.H, ho) : 0.0f;
   };
   for (int r = rounds - 1; r >= 0; --r) {
     float q[kScanStates];
@@ -656,12 +690,17 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   }
 
   const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
-  const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0 + c0;
-  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0 + c0;
-  const long long yb = (long long)p.b * a.L * a.H + p.h0 + c0;
+  const T* xp = static_cast<const T*>(a.x) + (long long)p.b * a.x_batch + p.h0;
+  const T* dp = static_cast<const T*>(a.dt) + (long long)p.b * a.dt_batch + p.h0;
+  const long long yb = (long long)p.b * a.L * a.H + p.h0;
   const T* gp = static_cast<const T*>(f.gy) + yb;
   T* gxp = static_cast<T*>(f.gx) + yb;
   T* gdp = static_cast<T*>(f.gdt) + yb;
+  float* pp = f.part_bc + ((long long)p.blk * a.B + p.b) * a.L * 2 * a.np;
+  const uint32_t xo = (uint32_t)(row * a.x_row + c0) * sizeof(T), dto = (uint32_t)(row * a.dt_row + c0) * sizeof(T);
+  const uint32_t oo = (uint32_t)(row * a.H + c0) * sizeof(T);
+  // what the folds leave in a lane: state lane / 32, token lane / 2 % 16, B or C
+  const uint32_t po = (uint32_t)(((lane >> 1 & 15) * 2 + (lane & 1)) * a.np + (lane >> 5)) * sizeof(float);
   float bias[kScanCols], dskip[kScanCols], gd[kScanCols] = {}, gbias[kScanCols] = {};
 #pragma unroll
   for (int i = 0; i < kScanCols; ++i) {
@@ -669,37 +708,36 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
     dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
   }
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile) {
-    const int t = tile * kScanTile + row;
-    if (t >= a.L) continue;
-    store_few<VEC, kScanCols>(gxp + (long long)t * a.H, cn, zero);
-    store_few<VEC, kScanCols>(gdp + (long long)t * a.H, cn, zero);
+    if (tile * kScanTile + row >= a.L) continue;
+    const long long at = (long long)tile * kScanTile * a.H;
+    store_few<VEC, kScanCols>(lane_at(gxp + at, oo), cn, zero);
+    store_few<VEC, kScanCols>(lane_at(gdp + at, oo), cn, zero);
   }
   Few<T, kScanCols, VEC> xv, dv, gv;
   auto fetch = [&](int tile) {
-    const int t = tile * kScanTile + row;
-    const int n = t < len ? cn : 0;
-    fetch_few(xp + (n > 0 ? t * a.x_row : 0), n, xv);
-    fetch_few(dp + (n > 0 ? t * a.dt_row : 0), n, dv);
-    fetch_few(gp + (n > 0 ? (long long)t * a.H : 0), n, gv);
+    xv = {}, dv = {}, gv = {};
+    if (tile * kScanTile + row < len && cn > 0) {
+      fetch_few(lane_at(xp + (long long)tile * kScanTile * a.x_row, xo), cn, xv);
+      fetch_few(lane_at(dp + (long long)tile * kScanTile * a.dt_row, dto), cn, dv);
+      fetch_few(lane_at(gp + (long long)tile * kScanTile * a.H, oo), cn, gv);
+    }
   };
-  const size_t pair = (size_t)a.ntiles * kScanTile * 4;
+  const size_t pair = (size_t)a.ntiles * kScanTile * 4;  // floats of two states
   const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
-  auto group_at = [&](int tile, int r, int g) {
-    return bc + r * kScanWaves * pair + ((size_t)tile * kGroups + g) * kScanGroup * 4;
-  };
-  BcGroup next;
+  auto tile_at = [&](int tile, int r) { return bc + r * kScanWaves * pair + (size_t)tile * kScanTile * 4; };
+  BcHalf next;
   u16s nextb = {};
   if (p.first < last) {
-    nextb = load_uniform(group_at(last - 1, 0, 0));
+    nextb = load_uniform<u16s>(tile_at(last - 1, 0));
     fetch(last - 1);
     load_saved(last - 1, 0, s0);
   }
   wait_loads();
   for (int tile = last - 1; tile >= p.first; --tile) {
     const int t0 = tile * kScanTile;
-    const bool in = t0 + row < len;  // tokens past the end change nothing
+    const bool in = t0 + row < len;
     float d[kScanCols], sg[kScanCols];
-    Few<T, kScanCols, VEC> xk = xv, gk = gv;
+    const Few<T, kScanCols, VEC> xk = xv, gk = gv;
 #pragma unroll
     for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[i], sg[i] = 1.0f;
     if (a.softplus) {
@@ -708,31 +746,33 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
     }
 #pragma unroll
     for (int i = 0; i < kScanCols; ++i) {
-      du[row][c0 + i] = in ? make_float2(d[i], d[i] * at_few(xk, i)) : make_float2(0.0f, 0.0f);
-      gys[row][c0 + i] = in ? at_few(gk, i) : 0.0f;
+      d[i] = in ? d[i] : 0.0f;  // past the end nothing changes
+      du[row][c0 + i] = make_float2(d[i], d[i] * at_few(xk, i));
+      gys[row][c0 + i] = at_few(gk, i);
     }
     if (tile > p.first) fetch(tile - 1);
     __syncthreads();
+    float s1[kScanTile], s2[kScanTile];  // sums over a wave's states
     for (int r = 0; r < rounds; ++r) {
       float s[kScanTile + 1][kScanStates], e[kScanTile][kScanStates], q[kScanStates], a3[kScanStates];
       const bool more = r + 1 < rounds;
-      const int tile2 = more ? tile : tile > p.first ? tile - 1 : tile, r2 = more ? r + 1 : 0;
+      const int tile2 = more || tile == p.first ? tile : tile - 1, r2 = more ? r + 1 : 0;
 #pragma unroll
       for (int i = 0; i < kScanStates; ++i) s[0][i] = s0[i];
       load_saved(tile2, r2, s0);
       if (MANY) load_rates(a, mine, h, r2, wave, a3);
-      // Forward with B alone, then back with both: the last group is first.
+      // Forward with B alone, then back with both.
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         float2 w[kScanGroup];
 #pragma unroll
         for (int j = 0; j < kScanGroup; ++j) w[j] = du[g * kScanGroup + j][lane];
-        wait_groups();
+        wait_scalars();
         const u16s now = nextb;
         if (g + 1 < kGroups)
-          nextb = load_uniform(group_at(tile, r, g + 1));
+          nextb = load_uniform<u16s>(tile_at(tile, r) + (g + 1) * 4 * kScanGroup);
         else
-          next = load_group(group_at(tile, r, g));
+          next = load_half(tile_at(tile, r), kHalves - 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kScanGroup; ++j) {
@@ -749,42 +789,37 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
       float rb[kScanTile], rc[kScanTile], ga[kScanStates] = {};
       qs.get(r, q);
 #pragma unroll
-      for (int g = kGroups - 1; g >= 0; --g) {
-        float2 w[kScanGroup];
-        float gyt[kScanGroup], o1[kScanGroup], o2[kScanGroup];
+      for (int g = kHalves - 1; g >= 0; --g) {
+        float2 w[kScanHalf];
+        float gyt[kScanHalf];
 #pragma unroll
-        for (int j = 0; j < kScanGroup; ++j) {
-          const int t = g * kScanGroup + j;
-          w[j] = du[t][lane], gyt[j] = gys[t][lane];
-          o1[j] = o2[j] = 0.0f;
-          if (MANY && r > 0) o1[j] = p1[wave][t][lane], o2[j] = p2[wave][t][lane];
-        }
-        wait_groups();
-        const BcGroup now = next;
+        for (int j = 0; j < kScanHalf; ++j) w[j] = du[g * kScanHalf + j][lane], gyt[j] = gys[g * kScanHalf + j][lane];
+        wait_scalars();
+        const BcHalf now = next;
         if (g > 0)
-          next = load_group(group_at(tile, r, g - 1));
-        else
-          nextb = load_uniform(group_at(tile2, r2, 0));
+          next = load_half(tile_at(tile, r), g - 1);
+        else  // of the next round or tile; the last one's own again
+          nextb = load_uniform<u16s>(tile_at(tile2, r2));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = kScanGroup - 1; j >= 0; --j) {
-          const int t = g * kScanGroup + j;
+        for (int j = kScanHalf - 1; j >= 0; --j) {
+          const int t = g * kScanHalf + j;
           float vb[kScanStates], vc[kScanStates];
+          if (!MANY || r == 0) s1[t] = s2[t] = 0.0f;
 #pragma unroll
           for (int i = 0; i < kScanStates; ++i) {
             const float G = fmaf(now.c(j, i), gyt[j], q[i]);
-            o1[j] = fmaf(now.b(j, i), G, o1[j]);
+            s1[t] = fmaf(now.b(j, i), G, s1[t]);
             vb[i] = G * w[j].y;
             vc[i] = gyt[j] * s[t + 1][i];
             q[i] = G * e[t][i];
             const float k = q[i] * s[t][i];
-            o2[j] = fmaf(k, a2[i], o2[j]);
+            s2[t] = fmaf(k, a2[i], s2[t]);
             ga[i] = fmaf(k, w[j].x, ga[i]);
           }
           rb[t] = fold32(vb[0], vb[1]);
           rc[t] = fold32(vc[0], vc[1]);
-          p1[wave][t][lane] = o1[j];
-          p2[wave][t][lane] = o2[j];
+          if (!MANY || !more) p1[wave][t][lane] = s1[t], p2[wave][t][lane] = s2[t];
           if (t < 8) {
             rb[t] = fold16(rb[t], rb[t + 8]);
             rc[t] = fold16(rc[t], rc[t + 8]);
@@ -810,19 +845,15 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
       rb[0] = fold_row<kDppXor2>(rb[0], rb[1], lane & 2);
       rc[0] = fold_row<kDppXor2>(rc[0], rc[1], lane & 2);
       rb[0] = fold_row<kDppXor1>(rb[0], rc[0], lane & 1);
-      // lane: state lane / 32, token lane / 2 % 16, B or C
-      const int t = t0 + (lane >> 1 & 15);
-      if (t < len)
-        f.part_bc[((((long long)p.blk * a.B + p.b) * a.L + t) * 2 + (lane & 1)) * a.np +
-                  (r * kScanWaves + wave) * kScanStates + (lane >> 5)] = rb[0];
+      if (t0 + (lane >> 1 & 15) < len)
+        *lane_at(pp + (long long)t0 * 2 * a.np + (r * kScanWaves + wave) * kScanStates, po) = rb[0];
       if (MANY) {
 #pragma unroll
         for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
       }
     }
     __syncthreads();
-    const int t = t0 + row;
-    if (t < a.L) {
+    if (t0 + row < a.L) {
       float ox[kScanCols], od[kScanCols];
 #pragma unroll
       for (int i = 0; i < kScanCols; ++i) {
@@ -835,8 +866,9 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
         gd[i] = fmaf(gy, x, gd[i]);
         gbias[i] += od[i];
       }
-      store_few<VEC, kScanCols>(gxp + (long long)t * a.H, cn, ox);
-      store_few<VEC, kScanCols>(gdp + (long long)t * a.H, cn, od);
+      const long long at = (long long)t0 * a.H;
+      store_few<VEC, kScanCols>(lane_at(gxp + at, oo), cn, ox);
+      store_few<VEC, kScanCols>(lane_at(gdp + at, oo), cn, od);
     }
     __syncthreads();
   }

@@ -96,6 +96,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _near_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` as the scan takes it: rows also less than 2^25 values apart."""
+    t = _rows(t)
+    return t if t.ndim < 3 or 0 <= t.stride(1) < 1 << 25 else t.contiguous()
+
+
 def _strides(t: torch.Tensor, n: int) -> list[int]:
     """The first n strides in elements; 0 along a dimension of one."""
     return [s if k > 1 else 0 for s, k in zip(t.stride()[:n], t.shape)]
@@ -297,7 +303,7 @@ class SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: Any, gy, gout=None):
         x, dt, A, b, c, D, dt_bias, state, lengths, saved = _saved(ctx)
-        x, dt = _rows(x), _rows(dt)
+        x, dt = _near_rows(x), _near_rows(dt)
         b, c = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (b, c))
         A, D, dt_bias, state, lengths, saved = (
             t if t is None else t.contiguous() for t in (A, D, dt_bias, state, lengths, saved))
@@ -333,7 +339,7 @@ def _check_scan(x, dt, A, B, C, D, dt_bias):
     shape = (*x.shape[:-1], B.shape[-2], N)
     _like(B, x, shape, "B")
     _like(C, x, shape, "C")
-    return _rows(x), _rows(dt), A, _rows(B), _rows(C), D, dt_bias
+    return _near_rows(x), _near_rows(dt), A, _rows(B), _rows(C), D, dt_bias
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
