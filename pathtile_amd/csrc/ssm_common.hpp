@@ -87,4 +87,27 @@ __device__ __forceinline__ float silu_grad_f32(float p, float sig) {
   return sig * fmaf(p, 1.0f - sig, 1.0f);
 }
 
+// Sums of columns over `parts` rows in a fixed order: 32 columns by 32 ranges of
+// rows a workgroup of 1024. column(i, &stride) is where column i begins, or
+// null, and sets how far its rows are apart; done(i, sum) takes the result.
+constexpr int kSumThreads = 1024, kSumCols = 32;
+template <typename Column, typename Done>
+__device__ __forceinline__ void sum_columns(long long first, long long parts, Column column, Done done) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+  long long stride = 0;
+  const float* p = column(first + c, &stride);
+  float v = 0.0f;
+  if (p) {
+#pragma unroll 8
+    for (long long i = k; i < parts; i += 32) v += p[i * stride];
+  }
+  sums[k][c] = v;
+  __syncthreads();
+  v = sums[c][k];
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v += __shfl_xor(v, m);
+  if (c == 0) done(first + k, v);
+}
+
 }  // namespace pt

@@ -33,28 +33,26 @@ struct CausalStep {
   static const void* fn() { return (const void*)&causal_step_kernel<T, V, K>; }
 };
 
-// gw [H, K] and gbias [H] from the runs' parts [parts][H][K + 1], 64 columns
-// by 4 ranges of parts a workgroup.
-__global__ __launch_bounds__(256) void causal_reduce_kernel(const float* __restrict__ part,
-                                                            float* __restrict__ gw,
-                                                            float* __restrict__ gbias,
-                                                            long long parts, int H, int K) {
-  __shared__ float sums[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long long cols = (long long)H * (K + 1), c = (long long)blockIdx.x * 64 + lane;
-  float v = 0.0f;
-  if (c < cols)
-    for (long long k = w; k < parts; k += 4) v += part[k * cols + c];
-  sums[w][lane] = v;
-  __syncthreads();
-  if (w || c >= cols) return;
-  v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-  const long long h = c / (K + 1);
-  const int j = (int)(c - h * (K + 1));
-  if (j < K)
-    gw[h * K + j] = v;
-  else if (gbias)
-    gbias[h] = v;
+// gw [H, K] and gbias [H] from the runs' parts [parts][H][K + 1].
+__global__ __launch_bounds__(kSumThreads) void causal_reduce_kernel(const float* __restrict__ part,
+                                                                    float* __restrict__ gw,
+                                                                    float* __restrict__ gbias,
+                                                                    long long parts, int H, int K) {
+  const long long cols = (long long)H * (K + 1);
+  sum_columns((long long)blockIdx.x * kSumCols, parts,
+              [&](long long c, long long* stride) {
+                *stride = cols;
+                return c < cols ? part + c : nullptr;
+              },
+              [&](long long c, float v) {
+                const long long h = c / (K + 1);
+                const int j = (int)(c - h * (K + 1));
+                if (c >= cols) return;
+                if (j < K)
+                  gw[h * K + j] = v;
+                else if (gbias)
+                  gbias[h] = v;
+              });
 }
 
 static int check_causal(int dtype, int B, int L, int H, int K) {
@@ -143,7 +141,8 @@ int pt_causal_conv_bwd(int dtype, const void* x, long long x_batch, long long x_
   long long parts = (long long)B * g.f.nruns;
   void* rargs[] = {&g.part, &gw, &gbias, &parts, &H, &K};
   return pt::ssm_launch((const void*)&pt::causal_reduce_kernel,
-                        pt::ssm_ceil((long long)H * (K + 1), 64), 256, stream, rargs);
+                        pt::ssm_ceil((long long)H * (K + 1), pt::kSumCols), pt::kSumThreads, stream,
+                        rargs);
 }
 
 int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* w, const float* bias,

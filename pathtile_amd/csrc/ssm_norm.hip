@@ -11,24 +11,29 @@ struct NormForm {
   bool vec;
 };
 
-// A wave up to 1024 channels, four up to 4096, sixteen up to 16384, with 8 or
-// 16 values a lane.
+// Eight values a lane, and as many lanes as a row needs; sixteen values from
+// 8192 channels on. More values a lane cost registers: at 4096 channels the
+// gated backward with the next row under way takes 216 for 16 and 126 for 8.
 static NormForm norm_form(int h, bool vec) {
-  NormForm f = {h <= 1024 ? 64 : h <= 4096 ? 256 : 1024, 16, vec};
-  if (f.tpr * 8 >= h) f.e = 8;
+  NormForm f = {64, 8, vec};
+  while (f.tpr * 8 < h && f.tpr < 1024) f.tpr *= 2;
+  if (f.tpr * 8 < h) f.e = 16;
   return f;
 }
 
+template <template <int, int, bool> class F, bool VEC>
+static const void* norm_of_form(const NormForm& f) {
+  switch (f.tpr) {
+    case 64: return F<8, 64, VEC>::fn();
+    case 128: return F<8, 128, VEC>::fn();
+    case 256: return F<8, 256, VEC>::fn();
+    case 512: return F<8, 512, VEC>::fn();
+    default: return f.e == 8 ? F<8, 1024, VEC>::fn() : F<16, 1024, VEC>::fn();
+  }
+}
 template <template <int, int, bool> class F>
 static const void* norm_fn(const NormForm& f) {
-  if (f.vec) {
-    if (f.tpr == 64) return f.e == 8 ? F<8, 64, true>::fn() : F<16, 64, true>::fn();
-    if (f.tpr == 256) return f.e == 8 ? F<8, 256, true>::fn() : F<16, 256, true>::fn();
-    return f.e == 8 ? F<8, 1024, true>::fn() : F<16, 1024, true>::fn();
-  }
-  if (f.tpr == 64) return f.e == 8 ? F<8, 64, false>::fn() : F<16, 64, false>::fn();
-  if (f.tpr == 256) return f.e == 8 ? F<8, 256, false>::fn() : F<16, 256, false>::fn();
-  return f.e == 8 ? F<8, 1024, false>::fn() : F<16, 1024, false>::fn();
+  return f.vec ? norm_of_form<F, true>(f) : norm_of_form<F, false>(f);
 }
 
 template <typename T>
@@ -62,12 +67,11 @@ static bool all16(const void* const* p, int n) {
   return true;
 }
 
-// Workgroups of a backward pass: four to a CU where a row takes four waves or
-// fewer, one where it takes sixteen, and no more than there are rows; a
-// multiple of what keeps a lane's rows in one group.
+// Workgroups of a backward pass: sixteen waves to a CU, and no more than there
+// are rows; a multiple of what keeps a lane's rows in one group.
 static long long norm_grid(long long rows, const NormForm& f, int groups) {
   const int per = norm_threads(f.tpr) / f.tpr;
-  long long n = f.tpr == 1024 ? 256 : 1024;
+  long long n = 256 * 1024 / norm_threads(f.tpr);
   if (n > ssm_ceil(rows, per)) n = ssm_ceil(rows, per);
   int g = groups, p = per;
   while (p) { const int r = g % p; g = p; p = r; }  // g = gcd(groups, per)
@@ -96,9 +100,9 @@ static long long residual_parts(long long rows, int H) {
   return norm_grid(rows, f, 1) * (norm_threads(f.tpr) / f.tpr);
 }
 
-static int sum_columns(const float* part, float* out, long long parts, int cols, void* stream) {
+static int launch_sums(const float* part, float* out, long long parts, int cols, void* stream) {
   void* args[] = {&part, &out, &parts, &cols};
-  return ssm_launch((const void*)&column_sum_kernel, ssm_ceil(cols, 64), 256, stream, args);
+  return ssm_launch((const void*)&column_sum_kernel, ssm_ceil(cols, kSumCols), kSumThreads, stream, args);
 }
 
 }  // namespace pt
@@ -141,7 +145,7 @@ int pt_gated_norm_bwd(int dtype, const void* x, long long x_row, const void* gat
   if (st != PT_OK) return st;
   if (!gw) return PT_ERR_NULL;
   float* part = static_cast<float*>(workspace);
-  if (rows == 0) return pt::sum_columns(part, gw, 0, H, stream);
+  if (rows == 0) return pt::launch_sums(part, gw, 0, H, stream);
   if (!x || !gate || !w || !rstd || !gy || !gx || !ggate) return PT_ERR_NULL;
   if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
   const int hg = H / groups;
@@ -157,7 +161,7 @@ int pt_gated_norm_bwd(int dtype, const void* x, long long x_row, const void* gat
   void* args[] = {&g};
   st = pt::ssm_launch(fn, pt::norm_grid(g.f.rows, f, groups), pt::norm_threads(f.tpr), stream, args);
   if (st != PT_OK) return st;
-  return pt::sum_columns(part, gw, pt::gated_parts(rows, H, groups), H, stream);
+  return pt::launch_sums(part, gw, pt::gated_parts(rows, H, groups), H, stream);
 }
 
 int pt_residual_norm_fwd(int dtype, int res_dtype, const void* x, long long x_row,
@@ -203,7 +207,7 @@ int pt_residual_norm_bwd(int dtype, int res_dtype, const void* x, long long x_ro
   if (st != PT_OK) return st;
   if (!gparams) return PT_ERR_NULL;
   float* part = static_cast<float*>(workspace);
-  if (rows == 0) return pt::sum_columns(part, gparams, 0, sums * H, stream);
+  if (rows == 0) return pt::launch_sums(part, gparams, 0, sums * H, stream);
   if (!x || !w || !rstd || (post_w && !rstd_x) || !gy || !gx) return PT_ERR_NULL;
   if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
   const void* ptrs[] = {x, residual, post_w, scale, w, gy, gsum, gx, gresidual, workspace};
@@ -219,7 +223,7 @@ int pt_residual_norm_bwd(int dtype, int res_dtype, const void* x, long long x_ro
   void* args[] = {&g};
   st = pt::ssm_launch(fn, pt::norm_grid(rows, f, 1), pt::norm_threads(f.tpr), stream, args);
   if (st != PT_OK) return st;
-  return pt::sum_columns(part, gparams, pt::residual_parts(rows, H), sums * H, stream);
+  return pt::launch_sums(part, gparams, pt::residual_parts(rows, H), sums * H, stream);
 }
 
 }  // extern "C"

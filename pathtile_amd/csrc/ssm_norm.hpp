@@ -19,8 +19,9 @@
 namespace pt {
 
 constexpr int kNormMaxH = 16384;
-// Lanes of a workgroup whose rows take TPR lanes each.
-constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+// Lanes of a workgroup whose rows take TPR lanes each: four rows of a wave, or
+// one row, so that a barrier never waits for another row.
+constexpr int norm_threads(int tpr) { return tpr > 64 ? tpr : 256; }
 
 struct NormArgs {
   const void *x, *z;        // [rows, H]; z: the gate
@@ -58,6 +59,43 @@ __device__ __forceinline__ void norm_load(const T* p, int l, int n, float (&v)[E
     }
   }
 }
+// The same values as they are in memory, for a row that is asked for while
+// another is worked on.
+template <typename T, int E, int TPR, bool VEC>
+struct RowAhead {
+  T v[E];
+  __device__ __forceinline__ void fetch(const T* p, int l, int n) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = norm_col<E, TPR, VEC>(l, i);
+      v[i] = c < n ? p[c] : (T)0.0f;
+    }
+  }
+  __device__ __forceinline__ void get(float (&o)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = (float)v[i];
+  }
+};
+template <typename T, int E, int TPR>
+struct RowAhead<T, E, TPR, true> {
+  static constexpr int kPieces = E * sizeof(T) / 16, kPer = 16 / sizeof(T);
+  u4v v[kPieces];
+  __device__ __forceinline__ void fetch(const T* p, int l, int n) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int c = norm_col<E, TPR, true>(l, i * kPer);
+      v[i] = u4v{0, 0, 0, 0};
+      if (c < n) v[i] = *reinterpret_cast<const u4v*>(p + c);
+    }
+  }
+  __device__ __forceinline__ void get(float (&o)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const uint32_t u = v[i / kPer][i % kPer * sizeof(T) / 4];
+      o[i] = sizeof(T) == 4 ? __uint_as_float(u) : i & 1 ? bf16_hi(u) : bf16_lo(u);
+    }
+  }
+};
 template <int E, int TPR, bool VEC, typename T>
 __device__ __forceinline__ void norm_store(T* p, int l, int n, const float (&v)[E]) {
   if constexpr (VEC) {
@@ -188,15 +226,24 @@ __global__ __launch_bounds__(norm_threads(TPR)) void gated_bwd_kernel(NormGradAr
   const long long first = (long long)blockIdx.x * kRows + sub;
   const long long step = (long long)gridDim.x * kRows;
   const int grp = (int)(first % a.groups), c0 = grp * a.hg;
-  float w[E], gw[E] = {};
+  float w[E], gw[E] = {}, r2 = 0.0f;
   norm_load<E, TPR, VEC>(a.w + c0, l, a.hg, w);
+  RowAhead<T, E, TPR, VEC> xa, za, ga;
+  auto fetch = [&](long long id) {
+    if (id >= a.rows) return;
+    const long long row = id / a.groups;
+    xa.fetch(static_cast<const T*>(a.x) + row * a.x_row + c0, l, a.hg);
+    za.fetch(static_cast<const T*>(a.z) + row * a.z_row + c0, l, a.hg);
+    ga.fetch(static_cast<const T*>(g.gy) + row * a.H + c0, l, a.hg);
+    r2 = a.rstd[id];
+  };
+  fetch(first);
   for (long long id = first; id < a.rows; id += step) {
     const long long row = id / a.groups;
+    const float r = r2;
     float x[E], z[E], gy[E], sum = 0.0f;
-    norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row + c0, l, a.hg, x);
-    norm_load<E, TPR, VEC>(static_cast<const T*>(a.z) + row * a.z_row + c0, l, a.hg, z);
-    norm_load<E, TPR, VEC>(static_cast<const T*>(g.gy) + row * a.H + c0, l, a.hg, gy);
-    const float r = a.rstd[id];
+    xa.get(x), za.get(z), ga.get(gy);
+    fetch(id + step);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const float n = x[i] * (z[i] * sigmoid_f32(z[i])) * r;
@@ -231,23 +278,32 @@ __global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGra
   constexpr int kRows = norm_threads(TPR) / TPR;
   const long long first = (long long)blockIdx.x * kRows + sub;
   const long long step = (long long)gridDim.x * kRows;
-  float gw[E] = {}, gs[E] = {}, gp[E] = {};
+  float gw[E] = {}, gs[E] = {}, gp[E] = {}, rr2 = 0.0f, rx2 = 1.0f;
+  RowAhead<T, E, TPR, VEC> xa, ga;
+  RowAhead<RT, E, TPR, VEC> ra, gra;
+  auto fetch = [&](long long row) {
+    if (row >= a.rows) return;
+    xa.fetch(static_cast<const T*>(a.x) + row * a.x_row, l, a.H);
+    ga.fetch(static_cast<const T*>(g.gy) + row * a.H, l, a.H);
+    if (a.residual) ra.fetch(static_cast<const RT*>(a.residual) + row * a.res_row, l, a.H);
+    if (g.gr) gra.fetch(static_cast<const RT*>(g.gr) + row * a.H, l, a.H);
+    rr2 = a.rstd[row];
+    if (a.pw) rx2 = a.rstd_x[row];
+  };
+  fetch(first);
   for (long long row = first; row < a.rows; row += step) {
-    float n[E], v[E], gy[E], w[E], sum = 0.0f, rx = 1.0f;
-    norm_load<E, TPR, VEC>(static_cast<const T*>(a.x) + row * a.x_row, l, a.H, n);
-    norm_load<E, TPR, VEC>(static_cast<const T*>(g.gy) + row * a.H, l, a.H, gy);
-    if (a.residual)
-      norm_load<E, TPR, VEC>(static_cast<const RT*>(a.residual) + row * a.res_row, l, a.H, v);
-    else {
+    float n[E], v[E], gy[E], gr[E], w[E], sum = 0.0f;
+    const float rr = rr2, rx = rx2;
+    xa.get(n), ga.get(gy);
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = 0.0f;
-    }
-    const float rr = a.rstd[row];
+    for (int i = 0; i < E; ++i) v[i] = gr[i] = 0.0f;
+    if (a.residual) ra.get(v);
+    if (g.gr) gra.get(gr);
+    fetch(row + step);
     float f[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) f[i] = n[i];
     if (a.pw) {
-      rx = a.rstd_x[row];
       norm_load<E, TPR, VEC>(a.pw, l, a.H, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) n[i] *= rx, f[i] = n[i] * w[i];
@@ -270,12 +326,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGra
     }
     sum = row_sum<TPR>(sum, lds, turn) / (float)a.H;
 #pragma unroll
-    for (int i = 0; i < E; ++i) gy[i] = rr * (gy[i] - v[i] * sum);
-    if (g.gr) {
-      norm_load<E, TPR, VEC>(static_cast<const RT*>(g.gr) + row * a.H, l, a.H, v);
-#pragma unroll
-      for (int i = 0; i < E; ++i) gy[i] += v[i];
-    }
+    for (int i = 0; i < E; ++i) gy[i] = gr[i] + rr * (gy[i] - v[i] * sum);
     if (g.gres) norm_store<E, TPR, VEC>(static_cast<RT*>(g.gres) + row * a.H, l, a.H, gy);
     if (a.scale) {
       norm_load<E, TPR, VEC>(a.scale, l, a.H, w);
@@ -304,19 +355,18 @@ __global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGra
   if (a.pw) norm_store<E, TPR, VEC>(part + (long long)(np - 1) * a.H, l, a.H, gp);
 }
 
-// out[c] = sum over k of part[k][c], 64 columns by 4 ranges a workgroup.
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part,
-                                                         float* __restrict__ out, long long parts,
-                                                         int cols) {
-  __shared__ float sums[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = (int)blockIdx.x * 64 + lane;
-  float v = 0.0f;
-  if (c < cols)
-    for (long long k = w; k < parts; k += 4) v += part[k * cols + c];
-  sums[w][lane] = v;
-  __syncthreads();
-  if (w == 0 && c < cols) out[c] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+// out[c] = sum over k of part[k][c].
+__global__ __launch_bounds__(kSumThreads) void column_sum_kernel(const float* __restrict__ part,
+                                                                 float* __restrict__ out, long long parts,
+                                                                 int cols) {
+  sum_columns((long long)blockIdx.x * kSumCols, parts,
+              [&](long long c, long long* stride) {
+                *stride = cols;
+                return c < cols ? part + c : nullptr;
+              },
+              [&](long long c, float v) {
+                if (c < cols) out[c] = v;
+              });
 }
 
 }  // namespace pt

@@ -6,34 +6,26 @@
 
 namespace pt {
 
-// gA [H, N], gD and gdt_bias [H] from the sequences' parts: 64 columns (a
-// channel of one of the np + 2 sums) by 4 ranges of sequences a workgroup.
-__global__ __launch_bounds__(256) void scan_param_reduce_kernel(ScanArgs a, const float* __restrict__ part_a,
-                                                                const float* __restrict__ part_d,
-                                                                float* __restrict__ ga, float* __restrict__ gd,
-                                                                float* __restrict__ gbias, int parts) {
-  __shared__ float sums[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long long col = (long long)blockIdx.x * 64 + lane;
+// gA [H, N], gD and gdt_bias [H] from the sequences' parts.
+__global__ __launch_bounds__(kSumThreads) void scan_param_reduce_kernel(
+    ScanArgs a, const float* __restrict__ part_a, const float* __restrict__ part_d,
+    float* __restrict__ ga, float* __restrict__ gd, float* __restrict__ gbias, int parts) {
   const long long na = (long long)a.np * a.H, cols = na + 2LL * a.H;
-  float v = 0.0f;
-  if (col < cols) {
-    const float* q = col < na ? part_a + col : part_d + (col - na);
-    const long long stride = col < na ? na : 2LL * a.H;
-    for (int k = w; k < parts; k += 4) v += q[k * stride];
-  }
-  sums[w][lane] = v;
-  __syncthreads();
-  if (w || col >= cols) return;
-  v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-  if (col < na) {
-    const int n = (int)(col / a.H), h = (int)(col - (long long)n * a.H);
-    if (n < a.N) ga[(long long)h * a.N + n] = v;
-  } else {
-    const int h = (int)((col - na) % a.H);
-    float* o = col - na < a.H ? gd : gbias;
-    if (o) o[h] = v;
-  }
+  sum_columns((long long)blockIdx.x * kSumCols, parts,
+              [&](long long c, long long* stride) -> const float* {
+                *stride = c < na ? na : 2LL * a.H;
+                return c < na ? part_a + c : c < cols ? part_d + (c - na) : nullptr;
+              },
+              [&](long long c, float v) {
+                if (c < na) {
+                  const int n = (int)(c / a.H), h = (int)(c - (long long)n * a.H);
+                  if (n < a.N) ga[(long long)h * a.N + n] = v;
+                } else if (c < cols) {
+                  const int h = (int)((c - na) % a.H);
+                  float* o = c - na < a.H ? gd : gbias;
+                  if (o) o[h] = v;
+                }
+              });
 }
 
 static int check_scan(const pt_scan_inputs* in, int L) {
@@ -216,7 +208,8 @@ int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float*
   int parts = a.B * a.chunks;
   void* pargs[] = {&a, &part_a, &part_d, &ga, &gd, &gdt_bias, &parts};
   return pt::ssm_launch((const void*)&pt::scan_param_reduce_kernel,
-                        pt::ssm_ceil((long long)(a.np + 2) * a.H, 64), 256, stream, pargs);
+                        pt::ssm_ceil((long long)(a.np + 2) * a.H, pt::kSumCols), pt::kSumThreads, stream,
+                        pargs);
 }
 
 int pt_selective_scan_step(const pt_scan_inputs* in, float* state, const int* slots, int pool,
