@@ -67,11 +67,13 @@ static bool all16(const void* const* p, int n) {
   return true;
 }
 
-// Workgroups of a backward pass: sixteen waves to a CU, and no more than there
-// are rows; a multiple of what keeps a lane's rows in one group.
-static long long norm_grid(long long rows, const NormForm& f, int groups) {
+// Workgroups of a backward pass: as many waves to a CU as its registers allow
+// (a few more would wait for a second round), and no more than there are rows;
+// a multiple of what keeps a lane's rows in one group.
+constexpr int kGatedWaves = 16, kResidualWaves = 12;
+static long long norm_grid(long long rows, const NormForm& f, int groups, int waves) {
   const int per = norm_threads(f.tpr) / f.tpr;
-  long long n = 256 * 1024 / norm_threads(f.tpr);
+  long long n = 256 * waves * 64 / norm_threads(f.tpr);
   if (n > ssm_ceil(rows, per)) n = ssm_ceil(rows, per);
   int g = groups, p = per;
   while (p) { const int r = g % p; g = p; p = r; }  // g = gcd(groups, per)
@@ -93,11 +95,11 @@ static int check_residual(int dtype, int res_dtype, long long rows, int H) {
 // The parts' layout must not depend on alignment: the same workspace serves.
 static long long gated_parts(long long rows, int H, int groups) {
   const NormForm f = norm_form(H / groups, true);
-  return norm_grid(rows * groups, f, groups) * (norm_threads(f.tpr) / f.tpr) / groups;
+  return norm_grid(rows * groups, f, groups, kGatedWaves) * (norm_threads(f.tpr) / f.tpr) / groups;
 }
 static long long residual_parts(long long rows, int H) {
   const NormForm f = norm_form(H, true);
-  return norm_grid(rows, f, 1) * (norm_threads(f.tpr) / f.tpr);
+  return norm_grid(rows, f, 1, kResidualWaves) * (norm_threads(f.tpr) / f.tpr);
 }
 
 static int launch_sums(const float* part, float* out, long long parts, int cols, void* stream) {
@@ -159,7 +161,7 @@ int pt_gated_norm_bwd(int dtype, const void* x, long long x_row, const void* gat
   const void* fn = dtype == PT_F32 ? pt::norm_fn<pt::Gated<float>::Bwd>(f)
                                    : pt::norm_fn<pt::Gated<__bf16>::Bwd>(f);
   void* args[] = {&g};
-  st = pt::ssm_launch(fn, pt::norm_grid(g.f.rows, f, groups), pt::norm_threads(f.tpr), stream, args);
+  st = pt::ssm_launch(fn, pt::norm_grid(g.f.rows, f, groups, pt::kGatedWaves), pt::norm_threads(f.tpr), stream, args);
   if (st != PT_OK) return st;
   return pt::launch_sums(part, gw, pt::gated_parts(rows, H, groups), H, stream);
 }
@@ -221,7 +223,7 @@ int pt_residual_norm_bwd(int dtype, int res_dtype, const void* x, long long x_ro
                    : res_dtype == PT_F32 ? pt::norm_fn<pt::Residual<__bf16, float>::Bwd>(f)
                                          : pt::norm_fn<pt::Residual<__bf16, __bf16>::Bwd>(f);
   void* args[] = {&g};
-  st = pt::ssm_launch(fn, pt::norm_grid(rows, f, 1), pt::norm_threads(f.tpr), stream, args);
+  st = pt::ssm_launch(fn, pt::norm_grid(rows, f, 1, pt::kResidualWaves), pt::norm_threads(f.tpr), stream, args);
   if (st != PT_OK) return st;
   return pt::launch_sums(part, gparams, pt::residual_parts(rows, H), sums * H, stream);
 }

@@ -286,19 +286,18 @@ __global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGra
     xa.fetch(static_cast<const T*>(a.x) + row * a.x_row, l, a.H);
     ga.fetch(static_cast<const T*>(g.gy) + row * a.H, l, a.H);
     if (a.residual) ra.fetch(static_cast<const RT*>(a.residual) + row * a.res_row, l, a.H);
-    if (g.gr) gra.fetch(static_cast<const RT*>(g.gr) + row * a.H, l, a.H);
     rr2 = a.rstd[row];
     if (a.pw) rx2 = a.rstd_x[row];
   };
   fetch(first);
   for (long long row = first; row < a.rows; row += step) {
-    float n[E], v[E], gy[E], gr[E], w[E], sum = 0.0f;
+    float n[E], v[E], gy[E], w[E], sum = 0.0f;
     const float rr = rr2, rx = rx2;
     xa.get(n), ga.get(gy);
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = gr[i] = 0.0f;
+    for (int i = 0; i < E; ++i) v[i] = 0.0f;
     if (a.residual) ra.get(v);
-    if (g.gr) gra.get(gr);
+    if (g.gr) gra.fetch(static_cast<const RT*>(g.gr) + row * a.H, l, a.H);
     fetch(row + step);
     float f[E];
 #pragma unroll
@@ -326,7 +325,12 @@ __global__ __launch_bounds__(norm_threads(TPR)) void residual_bwd_kernel(NormGra
     }
     sum = row_sum<TPR>(sum, lds, turn) / (float)a.H;
 #pragma unroll
-    for (int i = 0; i < E; ++i) gy[i] = gr[i] + rr * (gy[i] - v[i] * sum);
+    for (int i = 0; i < E; ++i) gy[i] = rr * (gy[i] - v[i] * sum);
+    if (g.gr) {
+      gra.get(v);
+#pragma unroll
+      for (int i = 0; i < E; ++i) gy[i] += v[i];
+    }
     if (g.gres) norm_store<E, TPR, VEC>(static_cast<RT*>(g.gres) + row * a.H, l, a.H, gy);
     if (a.scale) {
       norm_load<E, TPR, VEC>(a.scale, l, a.H, w);
