@@ -6,11 +6,14 @@
 // with x[b, -(K-1) .. -1] the state [B, K-1, H] of earlier tokens (or 0).
 //
 // Bound by HBM: 2 K + 5 FLOP for one element read and one written. A lane owns
-// V neighbouring channels (16 bytes) and walks a run of tokens with the last
-// K - 1 of them in registers, so each element is loaded once but for the K - 1
-// before a run, which neighbouring runs share through L2.
+// V neighbouring channels and walks a run of tokens by fours, with the K - 1
+// before them in registers and the next four under way, so that each element is
+// loaded once but for the K - 1 before a run, which neighbouring runs share
+// through L2.
 
 #pragma once
+
+#include <type_traits>
 
 #include "ssm_common.hpp"
 
@@ -18,6 +21,7 @@ namespace pt {
 
 constexpr int kCausalMaxK = 8;
 constexpr int kCausalThreads = 256;
+constexpr int kCausalFwdStep = 4, kCausalBwdStep = 4;  // tokens at a time; a run is a multiple
 
 struct CausalArgs {
   const void* x;      // [B, L, H], rows of H contiguous channels
@@ -28,25 +32,51 @@ struct CausalArgs {
   void* y;            // [B, L, H] contiguous
   void* state_out;    // [B, K-1, H] or null
   long long x_batch, x_row;  // strides of x in elements
-  int B, L, H, silu;
+  int B, L, H;
   int run, nruns;     // tokens of a run, runs of a sequence
   int cols;           // lanes that cover a row: ceil(H / V)
 };
 
-// A lane's channels at `p`: V of them, or its one.
+// V channels of one token as they are in memory.
+template <typename T, int V>
+struct Cols {
+  __attribute__((ext_vector_type(V * sizeof(T) / 4))) uint32_t v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const decltype(v)*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(v)*>(p) = v; }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+    return i & 1 ? bf16_hi(v[i / 2]) : bf16_lo(v[i / 2]);
+  }
+  __device__ __forceinline__ void set(const float (&o)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (sizeof(T) == 4)
+        v[i] = __float_as_uint(o[i]), v[i + 1] = __float_as_uint(o[i + 1]);
+      else
+        v[i / 2] = bf16_pair(o[i], o[i + 1]);
+    }
+  }
+};
+template <typename T>
+struct Cols<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ float at(int) const { return (float)v; }
+  __device__ __forceinline__ void set(const float (&o)[1]) { v = (T)o[0]; }
+};
 template <int V, typename T>
 __device__ __forceinline__ void load_cols(const T* p, float (&v)[V]) {
-  if constexpr (V == 1)
-    v[0] = load1(p);
-  else
-    load_vec<V>(p, v);
+  Cols<T, V> c;
+  c.load(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = c.at(i);
 }
 template <int V, typename T>
 __device__ __forceinline__ void store_cols(T* p, const float (&v)[V]) {
-  if constexpr (V == 1)
-    store1(p, v[0]);
-  else
-    store_vec<V>(p, v);
+  Cols<T, V> c;
+  c.set(v);
+  c.store(p);
 }
 
 // Lane `id` of the grid: its first channel, sequence and run. Channels are
@@ -70,69 +100,98 @@ __device__ __forceinline__ int clamped_length(const int* lengths, int b, int L) 
   return n < 0 ? 0 : n < L ? n : L;
 }
 
-// The token `t` of a sequence (its state's for t < 0) at channels h .. h + V - 1.
-template <typename T, int V, int K>
-__device__ __forceinline__ void load_token(const CausalArgs& a, const T* xb, int b, int h, int t,
-                                           float (&v)[V]) {
-  if (t >= 0) {
-    load_cols<V>(xb + (long long)t * a.x_row + h, v);
-  } else if (a.state) {
-    load_cols<V>(static_cast<const T*>(a.state) + ((long long)b * (K - 1) + (K - 1) + t) * a.H + h, v);
-  } else {
+// U tokens from t on, those below `end`, rows `row` apart from p on; 0 past it.
+template <typename T, int V, int U>
+__device__ __forceinline__ void load_step(const T* p, long long row, int t, int end, Cols<T, V> (&c)[U]) {
+  if (t + U <= end) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = 0.0f;
+    for (int u = 0; u < U; ++u) c[u].load(p + u * row);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    c[u] = {};
+    if (t + u < end) c[u].load(p + u * row);
   }
 }
 
-template <typename T, int V, int K>
+// The K - 1 tokens before token t of a sequence, of its state or 0 before the
+// first.
+template <typename T, int V, int K, int W>
+__device__ __forceinline__ void load_before(const CausalArgs& a, const T* xb, int b, int h, int t,
+                                            float (&win)[W][V]) {
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    const int s = t - (K - 1) + j;
+    if (s >= 0) {
+      load_cols<V>(xb + (long long)s * a.x_row + h, win[j]);
+    } else if (a.state) {
+      load_cols<V>(static_cast<const T*>(a.state) + ((long long)b * (K - 1) + (K - 1) + s) * a.H + h, win[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[j][i] = 0.0f;
+    }
+  }
+}
+
+template <typename T, int V, int K, bool SILU>
 __global__ __launch_bounds__(kCausalThreads) void causal_fwd_kernel(CausalArgs a) {
+  constexpr int U = kCausalFwdStep;
   CausalPlace at;
   if (!causal_place((long long)blockIdx.x * kCausalThreads + threadIdx.x, a, V, &at)) return;
   const int len = clamped_length(a.lengths, at.b, a.L);
   const T* xb = static_cast<const T*>(a.x) + (long long)at.b * a.x_batch;
-  T* yb = static_cast<T*>(a.y) + (long long)at.b * a.L * a.H + at.h;
   const int t0 = at.r * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
   const int te = t1 < len ? t1 : len;  // tokens from te on are past the sequence's end
+  const T* xp = xb + (long long)t0 * a.x_row + at.h;
+  T* yp = static_cast<T*>(a.y) + ((long long)at.b * a.L + t0) * a.H + at.h;
+  Cols<T, V> ahead[U];
+  load_step(xp, a.x_row, t0, te, ahead);
 
-  // The run that the sequence ends in writes the state: the last K - 1 tokens.
-  if (K > 1 && a.state_out && at.r == (len > 0 ? (len - 1) / a.run : 0)) {
-    T* so = static_cast<T*>(a.state_out) + (long long)at.b * (K - 1) * a.H + at.h;
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-      float v[V];
-      load_token<T, V, K>(a, xb, at.b, at.h, len - (K - 1) + j, v);
-      store_cols<V>(so + (long long)j * a.H, v);
-    }
-  }
-
-  float w[K][V], bias[V], win[K][V];
+  float w[K][V], bias[V], win[K - 1 + U][V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     bias[i] = a.bias ? a.bias[at.h + i] : 0.0f;
 #pragma unroll
     for (int j = 0; j < K; ++j) w[j][i] = a.w[(long long)(at.h + i) * K + j];
   }
-  if (t0 < te) {
+  // The run that the sequence ends in writes the state: the last K - 1 tokens.
+  if (K > 1 && a.state_out && at.r == (len > 0 ? (len - 1) / a.run : 0)) {
+    T* so = static_cast<T*>(a.state_out) + (long long)at.b * (K - 1) * a.H + at.h;
+    load_before<T, V, K>(a, xb, at.b, at.h, len, win);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) load_token<T, V, K>(a, xb, at.b, at.h, t0 - (K - 1) + j, win[j]);
+    for (int j = 0; j < K - 1; ++j) store_cols<V>(so + (long long)j * a.H, win[j]);
   }
-  const T* xp = xb + (long long)t0 * a.x_row + at.h;
-  for (int t = t0; t < te; ++t, xp += a.x_row) {
-    load_cols<V>(xp, win[K - 1]);
-    float y[V];
+  if (t0 < te) load_before<T, V, K>(a, xb, at.b, at.h, t0, win);
+  for (int t = t0; t < te; t += U) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float p = bias[i];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < K; ++j) p = fmaf(w[j][i], win[j][i], p);
-      y[i] = a.silu ? p * sigmoid_f32(p) : p;
+      for (int i = 0; i < V; ++i) win[K - 1 + u][i] = ahead[u].at(i);
+    xp += U * a.x_row;
+    load_step(xp, a.x_row, t + U, te, ahead);
+    float y[U][V];
 #pragma unroll
-      for (int j = 0; j + 1 < K; ++j) win[j][i] = win[j + 1][i];
-    }
-    store_cols<V>(yb + (long long)t * a.H, y);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        y[u][i] = bias[i];
+#pragma unroll
+        for (int j = 0; j < K; ++j) y[u][i] = fmaf(w[j][i], win[u + j][i], y[u][i]);
+        if (SILU) y[u][i] *= sigmoid_f32(y[u][i]);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < te) store_cols<V>(yp + (long long)u * a.H, y[u]);
+    yp += (long long)U * a.H;
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[j][i] = win[j + U][i];
   }
-  float zero[V] = {};
-  for (int t = te > t0 ? te : t0; t < t1; ++t) store_cols<V>(yb + (long long)t * a.H, zero);
+  const float zero[V] = {};
+  T* zp = static_cast<T*>(a.y) + (long long)at.b * a.L * a.H + at.h;
+  for (int t = te > t0 ? te : t0; t < t1; ++t) store_cols<V>(zp + (long long)t * a.H, zero);
 }
 
 struct CausalGradArgs {
@@ -150,104 +209,120 @@ struct CausalGradArgs {
 // it sums dw over its own tokens alone, and writes gx K - 1 tokens behind. The
 // first run also writes the initial state's gradient, gx at t < 0. A final
 // state's gradient adds to gx at the last K - 1 tokens.
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool SILU>
 __global__ __launch_bounds__(kCausalThreads) void causal_bwd_kernel(CausalGradArgs g) {
+  constexpr int U = kCausalBwdStep;
   const CausalArgs& a = g.f;
   CausalPlace at;
   if (!causal_place((long long)blockIdx.x * kCausalThreads + threadIdx.x, a, V, &at)) return;
   const int len = clamped_length(a.lengths, at.b, a.L);
   const T* xb = static_cast<const T*>(a.x) + (long long)at.b * a.x_batch;
-  const T* gyb = static_cast<const T*>(g.gy) + (long long)at.b * a.L * a.H + at.h;
   const T* gsb = static_cast<const T*>(g.gstate) + (long long)at.b * (K - 1) * a.H + at.h;
-  T* gxb = static_cast<T*>(g.gx) + (long long)at.b * a.L * a.H + at.h;
   T* gib = static_cast<T*>(g.gstate_in) + (long long)at.b * (K - 1) * a.H + at.h;
   const int t0 = at.r * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
+  const T* xp = xb + (long long)t0 * a.x_row + at.h;
+  const T* gp = static_cast<const T*>(g.gy) + ((long long)at.b * a.L + t0) * a.H + at.h;
+  T* gxp = static_cast<T*>(g.gx) + ((long long)at.b * a.L + t0 - (K - 1)) * a.H + at.h;
+  // Tokens from te on have a dp of 0.
+  const int te = t1 + K - 1 < len ? t1 + K - 1 : len;
+  Cols<T, V> xa[U], ga[U];
+  load_step(xp, a.x_row, t0, te, xa);
+  load_step(gp, a.H, t0, te, ga);
 
-  float w[K][V], bias[V], win[K][V], dp[K][V], dw[K][V] = {}, db[V] = {};
+  float w[K][V], bias[V], win[K - 1 + U][V], dp[K - 1 + U][V], dw[K][V] = {}, db[V] = {};
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     bias[i] = a.bias ? a.bias[at.h + i] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      w[j][i] = a.w[(long long)(at.h + i) * K + j];
-      dp[j][i] = win[j][i] = 0.0f;
-    }
+    for (int j = 0; j < K; ++j) w[j][i] = a.w[(long long)(at.h + i) * K + j];
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) dp[j][i] = win[j][i] = 0.0f;
   }
+  if (t0 < len) load_before<T, V, K>(a, xb, at.b, at.h, t0, win);
   // The first run starts K - 1 tokens early, where dp is 0: the gradients of
   // the state's tokens come out there.
-  const int first = at.r == 0 && K > 1 ? t0 - (K - 1) : t0;
-  if (t0 < len) {
+  const int first = at.r == 0 ? t0 - (K - 1) : t0;
+  // OWN: the run's tokens; WHOLE: inside the sequence, and so far from the run's
+  // ends that every gx is plain.
+  auto step = [&](int t, auto own, auto whole) {
+    constexpr bool OWN = decltype(own)::value, WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) load_token<T, V, K>(a, xb, at.b, at.h, t0 - (K - 1) + j, win[j]);
-  }
-  for (int t = t0; t < t1 + K - 1; ++t) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j + 1 < K; ++j)
+      for (int i = 0; i < V; ++i) win[K - 1 + u][i] = xa[u].at(i), dp[K - 1 + u][i] = ga[u].at(i);
+    xp += U * a.x_row, gp += (long long)U * a.H;
+    load_step(xp, a.x_row, t + U, te, xa);
+    load_step(gp, a.H, t + U, te, ga);
 #pragma unroll
-      for (int i = 0; i < V; ++i) dp[j][i] = dp[j + 1][i];
-    if (t < len) {
-      float gy[V];
-      load_cols<V>(xb + (long long)t * a.x_row + at.h, win[K - 1]);
-      load_cols<V>(gyb + (long long)t * a.H, gy);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float d = gy[i];
-        if (a.silu) {
+        float& d = dp[K - 1 + u][i];  // gy so far, 0 past the end
+        if (SILU) {
           float p = bias[i];
 #pragma unroll
-          for (int j = 0; j < K; ++j) p = fmaf(w[j][i], win[j][i], p);
-          d *= silu_grad_f32(p, sigmoid_f32(p));
+          for (int j = 0; j < K; ++j) p = fmaf(w[j][i], win[u + j][i], p);
+          const float grad = d * silu_grad_f32(p, sigmoid_f32(p));
+          d = WHOLE || t + u < te ? grad : 0.0f;
         }
-        dp[K - 1][i] = d;
-        if (t < t1) {
+        if (OWN) {
           db[i] += d;
 #pragma unroll
-          for (int j = 0; j < K; ++j) dw[j][i] = fmaf(d, win[j][i], dw[j][i]);
+          for (int j = 0; j < K; ++j) dw[j][i] = fmaf(d, win[u + j][i], dw[j][i]);
         }
-#pragma unroll
-        for (int j = 0; j + 1 < K; ++j) win[j][i] = win[j + 1][i];
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) dp[K - 1][i] = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      const int s = t + u - (K - 1);  // dp[u .. u + K - 1] are tokens s ..
+      float out[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        out[i] = w[0][i] * dp[u + K - 1][i];
+#pragma unroll
+        for (int j = 1; j < K; ++j) out[i] = fmaf(w[j][i], dp[u + K - 1 - j][i], out[i]);
+      }
+      if (!WHOLE) {
+        if (s < first || s >= t1) continue;
+        if (K > 1 && g.gstate && s >= len - (K - 1) && s < len) {
+          float v[V];
+          load_cols<V>(gsb + (long long)(s - (len - (K - 1))) * a.H, v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) out[i] += v[i];
+        }
+        if (s < 0) {
+          if (g.gstate_in) store_cols<V>(gib + (long long)(s + K - 1) * a.H, out);
+          continue;
+        }
+      }
+      store_cols<V>(gxp + (long long)u * a.H, out);
     }
-    const int s = t - (K - 1);  // dp holds tokens s .. t
-    if (s < first) continue;
-    float out[V];
+    gxp += (long long)U * a.H;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      out[i] = 0.0f;
+    for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-      for (int j = 0; j < K; ++j) out[i] = fmaf(w[j][i], dp[K - 1 - j][i], out[i]);
-    }
-    if (K > 1 && g.gstate && s >= len - (K - 1) && s < len) {
-      float v[V];
-      load_cols<V>(gsb + (long long)(s - (len - (K - 1))) * a.H, v);
+      for (int i = 0; i < V; ++i) win[j][i] = win[j + U][i], dp[j][i] = dp[j + U][i];
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  int t = t0;
+  for (; t < t0 + K - 1 && t < t1; t += U) step(t, yes, no);
+  for (const int e = t1 < len ? t1 : len; t + U <= e; t += U) step(t, yes, yes);
+  for (; t < t1; t += U) step(t, yes, no);
+  for (; t < t1 + K - 1; t += U) step(t, no, no);
+  float* part = g.part + ((long long)at.b * a.nruns + at.r) * (K + 1) * a.H + at.h;
 #pragma unroll
-      for (int i = 0; i < V; ++i) out[i] += v[i];
-    }
-    if (s >= 0)
-      store_cols<V>(gxb + (long long)s * a.H, out);
-    else if (g.gstate_in)
-      store_cols<V>(gib + (long long)(s + K - 1) * a.H, out);
-  }
-  float* part = g.part + (((long long)at.b * a.nruns + at.r) * a.H + at.h) * (K + 1);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) part[i * (K + 1) + j] = dw[j][i];
-    part[i * (K + 1) + K] = db[i];
-  }
+  for (int j = 0; j < K; ++j) store_cols<V>(part + (long long)j * a.H, dw[j]);
+  store_cols<V>(part + (long long)K * a.H, db);
 }
 
 // One token of each of B sequences: the pool's states shift by it in place.
 // slots (null: sequence b has state b): a slot outside the pool marks a row
 // without a sequence, whose y is 0.
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool SILU>
 __global__ __launch_bounds__(kCausalThreads) void causal_step_kernel(
     const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias,
     T* __restrict__ state, const int* __restrict__ slots, T* __restrict__ y, long long x_row,
-    int B, int H, int pool, int silu, int cols) {
+    int B, int H, int pool, int cols) {
   const long long id = (long long)blockIdx.x * kCausalThreads + threadIdx.x;
   const int b = (int)(id / cols), h = (int)(id - (long long)b * cols) * V;
   if (b >= B) return;
@@ -264,7 +339,7 @@ __global__ __launch_bounds__(kCausalThreads) void causal_step_kernel(
       float p = bias ? bias[h + i] : 0.0f;
 #pragma unroll
       for (int j = 0; j < K; ++j) p = fmaf(w[(long long)(h + i) * K + j], win[j][i], p);
-      out[i] = silu ? p * sigmoid_f32(p) : p;
+      out[i] = SILU ? p * sigmoid_f32(p) : p;
     }
 #pragma unroll
     for (int j = 0; j + 1 < K; ++j) store_cols<V>(sp + (long long)j * H, win[j + 1]);
