@@ -202,7 +202,7 @@ int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float*
     void* bargs[] = {&a, &cpart, &gb, &gc};
     st = pt::ssm_launch(in->dtype == PT_F32 ? (const void*)&pt::scan_bc_reduce_kernel<float>
                                             : (const void*)&pt::scan_bc_reduce_kernel<__bf16>,
-                        pt::ssm_ceil((long long)a.B * a.L * a.G * 2 * a.np, 256), 256, stream, bargs);
+                        pt::ssm_ceil((long long)a.B * a.L * a.G * (a.np / 2), 256), 256, stream, bargs);
     if (st != PT_OK) return st;
   }
   int parts = a.B * a.chunks;

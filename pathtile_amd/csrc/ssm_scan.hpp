@@ -460,7 +460,8 @@ template <typename T, bool MANY, bool VEC>
 __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   constexpr int kGroups = kScanTile / kScanGroup;
   __shared__ float2 du[2][kScanTile][kScanCh];
-  __shared__ float yp[2][kScanWaves][kScanTile][kScanCh];
+  // Many rounds: one buffer and a second barrier, and so two workgroups a CU.
+  __shared__ float yp[MANY ? 1 : 2][kScanWaves][kScanTile][kScanCh];
   __shared__ typename Rounds<MANY>::Lds hold;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   float a2[kScanStates];
   for (int r = rounds - 1; r >= 0; --r) {
     float s[kScanStates];
-    load_rates(a, mine, h, r, wave, a2);
+    if (r == 0 || p.c > 0) load_rates(a, mine, h, r, wave, a2);
     load_states(a.state, mine, a, (long long)p.b * a.H + h, r, wave, s);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, 0, p.c, r, wave, h, a2, s);
     states.set(r, s);
@@ -577,7 +578,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
       }
     }
 #pragma unroll
-    for (int t = 0; t < kScanTile; ++t) yp[buf][wave][t][lane] = y[t];
+    for (int t = 0; t < kScanTile; ++t) yp[MANY ? 0 : buf][wave][t][lane] = y[t];
     float xr[kScanCols];
 #pragma unroll
     for (int i = 0; i < kScanCols; ++i) xr[i] = xk[i];
@@ -593,11 +594,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
       for (int i = 0; i < kScanCols; ++i) {
         float v = dskip[i] * xr[i];
 #pragma unroll
-        for (int w = 0; w < kScanWaves; ++w) v += yp[buf][w][row][c0 + i];
+        for (int w = 0; w < kScanWaves; ++w) v += yp[MANY ? 0 : buf][w][row][c0 + i];
         out[i] = t < len ? v : 0.0f;
       }
       store_few<VEC, kScanCols>(lane_at(op + (long long)tile * kScanTile * a.H, oo), cn, out);
     }
+    if (MANY) __syncthreads();
   }
   const float zero[kScanCols] = {};
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile)
@@ -682,7 +684,7 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   };
   for (int r = rounds - 1; r >= 0; --r) {
     float q[kScanStates];
-    load_rates(a, mine, h, r, wave, a2);
+    if (r == 0 || p.c < a.chunks - 1) load_rates(a, mine, h, r, wave, a2);
     load_states(f.gstate_out, mine, a, (long long)p.b * a.H + h, r, wave, q);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, a.chunks - 1, p.c, r, wave, h, a2, q);
     qs.set(r, q);
@@ -894,24 +896,29 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   }
 }
 
-// gB, gC [B, L, G, N] from the blocks' parts.
+// gB, gC [B, L, G, N] from the blocks' parts, four states a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_reduce_kernel(ScanArgs a, const float* __restrict__ part,
                                                              T* __restrict__ gb, T* __restrict__ gc) {
+  const int lanes = a.np / 2;  // of one token: B's, then C's
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = id / (2 * a.np);  // (b L + t) G + g
+  const long long row = id / lanes;  // (b L + t) G + g
   if (row >= (long long)a.B * a.L * a.G) return;
-  const int r = (int)(id - row * 2 * a.np), half = r / a.np, n = r - half * a.np;
-  if (n >= a.N) return;
+  const int r = (int)(id - row * lanes) * 4, half = r / a.np, n = r - half * a.np;
   const int g = (int)(row % a.G);
   const long long bt = row / a.G;
   const int b = (int)(bt / a.L), t = (int)(bt - (long long)b * a.L);
-  float v = 0.0f;
+  f4v v = {0.0f, 0.0f, 0.0f, 0.0f};
   if (t < scan_length(a, b)) {
     const float* q = part + ((long long)g * a.blocks_g * a.B * a.L + bt) * 2 * a.np + r;
-    for (int k = 0; k < a.blocks_g; ++k, q += (long long)a.B * a.L * 2 * a.np) v += *q;
+#pragma unroll 4
+    for (int k = 0; k < a.blocks_g; ++k)
+      v += *reinterpret_cast<const f4v*>(q + (long long)k * a.B * a.L * 2 * a.np);
   }
-  store1((half ? gc : gb) + row * a.N + n, v);
+  T* o = (half ? gc : gb) + row * a.N + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < a.N) store1(o + i, v[i]);
 }
 
 // One token of each of B sequences, states of a pool updated in place. PER
