@@ -41,14 +41,14 @@ static int check_scan(const pt_scan_inputs* in, int L) {
   return in->x && in->dt && in->a && in->b && in->c ? PT_OK : PT_ERR_NULL;
 }
 
-// Tiles of a chunk: sequences are taken in one piece where there is a workgroup
-// for each of 256 CUs, and otherwise in pieces of at least eight tiles, two to
-// a CU. Fewer than three pieces do not pay for the pass that they need first.
+// Tiles of a chunk. A workgroup a CU keeps the chip busy from about 160 on (in
+// one piece 192 take 192 us and 128 take 189 at 2048 tokens of 16 states, in
+// chunks 225 and 160); fewer are cut into chunks of four tiles or more, two to
+// each of 256 CUs, which costs the pass for their states.
 static int scan_chunk_tiles(long long blocks, int ntiles) {
-  long long chunks = blocks >= 256 ? 1 : ssm_ceil(512, blocks);
-  if (chunks > ntiles / 8) chunks = ntiles / 8;
-  if (chunks < 3) chunks = 1;
-  return (int)ssm_ceil(ntiles, chunks);
+  long long chunks = blocks >= 160 ? 1 : ssm_ceil(512, blocks);
+  if (chunks > ntiles / 4) chunks = ntiles / 4;
+  return (int)ssm_ceil(ntiles, chunks > 1 ? chunks : 1);
 }
 
 static ScanArgs scan_args(const pt_scan_inputs* in) {

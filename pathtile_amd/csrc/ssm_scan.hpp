@@ -658,11 +658,12 @@ __device__ __forceinline__ float fold_row(float u, float v, bool bit) {
 constexpr int kDppRor8 = 0x128, kDppHalfMirror = 0x141, kDppXor2 = 0x4e, kDppXor1 = 0xb1;
 
 template <typename T, bool MANY, bool VEC>
-__global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f) {
-  constexpr int kGroups = kScanTile / kScanGroup, kHalves = kScanTile / kScanHalf;
+__global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(ScanBwdArgs f) {
+  constexpr int kHalves = kScanTile / kScanHalf;
   __shared__ float2 du[kScanTile][kScanCh];
   __shared__ float gys[kScanTile][kScanCh];
   __shared__ float p1[kScanWaves][kScanTile][kScanCh], p2[kScanWaves][kScanTile][kScanCh];
+  __shared__ float bias[kScanCh], dskip[kScanCh];
   __shared__ typename Rounds<MANY>::Lds hold_q, hold_a;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
@@ -701,13 +702,14 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   float* pp = f.part_bc + ((long long)p.blk * a.B + p.b) * a.L * 2 * a.np;
   const uint32_t xo = (uint32_t)(row * a.x_row + c0) * sizeof(T), dto = (uint32_t)(row * a.dt_row + c0) * sizeof(T);
   const uint32_t oo = (uint32_t)(row * a.H + c0) * sizeof(T);
-  // what the folds leave in a lane: state lane / 32, token lane / 2 % 16, B or C
-  const uint32_t po = (uint32_t)(((lane >> 1 & 15) * 2 + (lane & 1)) * a.np + (lane >> 5)) * sizeof(float);
-  float bias[kScanCols], dskip[kScanCols], gd[kScanCols] = {}, gbias[kScanCols] = {};
-#pragma unroll
-  for (int i = 0; i < kScanCols; ++i) {
-    bias[i] = a.dt_bias && i < cn ? a.dt_bias[p.h0 + c0 + i] : 0.0f;
-    dskip[i] = a.d && i < cn ? a.d[p.h0 + c0 + i] : 0.0f;
+  // What the folds leave in a lane: state lane / 32, token of bits 4, 3, 2, 1, B
+  // or C.
+  const int pt = (lane >> 4 & 1) | (lane >> 2 & 2) | (lane & 4) | (lane << 2 & 8);
+  const uint32_t po = (uint32_t)((pt * 2 + (lane & 1)) * a.np + (lane >> 5)) * sizeof(float);
+  float gd[kScanCols] = {}, gbias[kScanCols] = {};
+  if (tid < kScanCh) {
+    bias[tid] = a.dt_bias && mine ? a.dt_bias[h] : 0.0f;
+    dskip[tid] = a.d && mine ? a.d[h] : 0.0f;
   }
   for (int tile = p.first > last ? p.first : last; tile < p.last; ++tile) {
     if (tile * kScanTile + row >= a.L) continue;
@@ -728,20 +730,21 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
   auto tile_at = [&](int tile, int r) { return bc + r * kScanWaves * pair + (size_t)tile * kScanTile * 4; };
   BcHalf next;
-  u16s nextb = {};
+  u16s nextb = {}, nowb;
   if (p.first < last) {
     nextb = load_uniform<u16s>(tile_at(last - 1, 0));
     fetch(last - 1);
     load_saved(last - 1, 0, s0);
   }
   wait_loads();
+  __syncthreads();
   for (int tile = last - 1; tile >= p.first; --tile) {
     const int t0 = tile * kScanTile;
     const bool in = t0 + row < len;
     float d[kScanCols], sg[kScanCols];
-    const Few<T, kScanCols, VEC> xk = xv, gk = gv;
+    const Few<T, kScanCols, VEC> xk = xv;
 #pragma unroll
-    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[i], sg[i] = 1.0f;
+    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[c0 + i], sg[i] = 1.0f;
     if (a.softplus) {
 #pragma unroll
       for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &sg[i]);
@@ -750,7 +753,7 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
     for (int i = 0; i < kScanCols; ++i) {
       d[i] = in ? d[i] : 0.0f;  // past the end nothing changes
       du[row][c0 + i] = make_float2(d[i], d[i] * at_few(xk, i));
-      gys[row][c0 + i] = at_few(gk, i);
+      gys[row][c0 + i] = at_few(gv, i);
     }
     if (tile > p.first) fetch(tile - 1);
     __syncthreads();
@@ -765,27 +768,29 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
       if (MANY) load_rates(a, mine, h, r2, wave, a3);
       // Forward with B alone, then back with both.
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        float2 w[kScanGroup];
+      for (int g = 0; g < kHalves; ++g) {
+        float2 w[kScanHalf];
 #pragma unroll
-        for (int j = 0; j < kScanGroup; ++j) w[j] = du[g * kScanGroup + j][lane];
-        wait_scalars();
-        const u16s now = nextb;
-        if (g + 1 < kGroups)
-          nextb = load_uniform<u16s>(tile_at(tile, r) + (g + 1) * 4 * kScanGroup);
-        else
-          next = load_half(tile_at(tile, r), kHalves - 1);
+        for (int j = 0; j < kScanHalf; ++j) w[j] = du[g * kScanHalf + j][lane];
+        if (g % 2 == 0) {
+          wait_scalars();
+          nowb = nextb;
+          if (g + 2 < kHalves)
+            nextb = load_uniform<u16s>(tile_at(tile, r) + (g / 2 + 1) * 4 * kScanGroup);
+          else
+            next = load_half(tile_at(tile, r), kHalves - 1);
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < kScanGroup; ++j) {
-          const int t = g * kScanGroup + j;
+        for (int j = 0; j < kScanHalf; ++j) {
+          const int t = g * kScanHalf + j;
 #pragma unroll
           for (int i = 0; i < kScanStates; ++i) {
             e[t][i] = __builtin_amdgcn_exp2f(w[j].x * a2[i]);
-            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(now, j, i));
+            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(nowb, g % 2 * kScanHalf + j, i));
           }
         }
-        pin(s[(g + 1) * kScanGroup]);
+        pin(s[(g + 1) * kScanHalf]);
         __builtin_amdgcn_sched_barrier(0);
       }
       float rb[kScanTile], rc[kScanTile], ga[kScanStates] = {};
@@ -822,13 +827,18 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
           rb[t] = fold32(vb[0], vb[1]);
           rc[t] = fold32(vc[0], vc[1]);
           if (!MANY || !more) p1[wave][t][lane] = s1[t], p2[wave][t][lane] = s2[t];
-          if (t < 8) {
-            rb[t] = fold16(rb[t], rb[t + 8]);
-            rc[t] = fold16(rc[t], rc[t + 8]);
+          // Neighbours first, so that few folds wait for their partner.
+          if (t % 2 == 0) {
+            rb[t] = fold16(rb[t], rb[t + 1]);
+            rc[t] = fold16(rc[t], rc[t + 1]);
           }
-          if (t < 4) {
-            rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 4], lane & 8);
-            rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 4], lane & 8);
+          if (t % 4 == 0) {
+            rb[t] = fold_row<kDppRor8>(rb[t], rb[t + 2], lane & 8);
+            rc[t] = fold_row<kDppRor8>(rc[t], rc[t + 2], lane & 8);
+          }
+          if (t % 8 == 0) {
+            rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 4], lane & 4);
+            rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 4], lane & 4);
           }
         }
         pin(q);
@@ -839,15 +849,10 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
 #pragma unroll
       for (int i = 0; i < kScanStates; ++i) ga[i] += q[i];
       gas.set(r, ga);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        rb[t] = fold_row<kDppHalfMirror>(rb[t], rb[t + 2], lane & 4);
-        rc[t] = fold_row<kDppHalfMirror>(rc[t], rc[t + 2], lane & 4);
-      }
-      rb[0] = fold_row<kDppXor2>(rb[0], rb[1], lane & 2);
-      rc[0] = fold_row<kDppXor2>(rc[0], rc[1], lane & 2);
+      rb[0] = fold_row<kDppXor2>(rb[0], rb[8], lane & 2);
+      rc[0] = fold_row<kDppXor2>(rc[0], rc[8], lane & 2);
       rb[0] = fold_row<kDppXor1>(rb[0], rc[0], lane & 1);
-      if (t0 + (lane >> 1 & 15) < len)
+      if (t0 + pt < len)
         *lane_at(pp + (long long)t0 * 2 * a.np + (r * kScanWaves + wave) * kScanStates, po) = rb[0];
       if (MANY) {
 #pragma unroll
@@ -862,8 +867,8 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
         float g1 = 0.0f, g2 = 0.0f;
 #pragma unroll
         for (int w = 0; w < kScanWaves; ++w) g1 += p1[w][row][c0 + i], g2 += p2[w][row][c0 + i];
-        const float x = at_few(xk, i), gy = at_few(gk, i);  // 0 past the end
-        ox[i] = in ? fmaf(d[i], g1, dskip[i] * gy) : 0.0f;
+        const float x = at_few(xk, i), gy = gys[row][c0 + i];  // 0 past the end
+        ox[i] = in ? fmaf(du[row][c0 + i].x, g1, dskip[c0 + i] * gy) : 0.0f;
         od[i] = in ? fmaf(x, g1, kLn2 * g2) * sg[i] : 0.0f;
         gd[i] = fmaf(gy, x, gd[i]);
         gbias[i] += od[i];
