@@ -660,6 +660,7 @@ constexpr int kDppRor8 = 0x128, kDppHalfMirror = 0x141, kDppXor2 = 0x4e, kDppXor
 template <typename T, bool MANY, bool VEC>
 __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(ScanBwdArgs f) {
   constexpr int kHalves = kScanTile / kScanHalf;
+  constexpr int kAhead = MANY ? kScanGroup : kScanHalf;  // tokens asked of LDS at a time
   __shared__ float2 du[kScanTile][kScanCh];
   __shared__ float gys[kScanTile][kScanCh];
   __shared__ float p1[kScanWaves][kScanTile][kScanCh], p2[kScanWaves][kScanTile][kScanCh];
@@ -768,29 +769,29 @@ __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(Sc
       if (MANY) load_rates(a, mine, h, r2, wave, a3);
       // Forward with B alone, then back with both.
 #pragma unroll
-      for (int g = 0; g < kHalves; ++g) {
-        float2 w[kScanHalf];
+      for (int g = 0; g < kScanTile / kAhead; ++g) {
+        float2 w[kAhead];
 #pragma unroll
-        for (int j = 0; j < kScanHalf; ++j) w[j] = du[g * kScanHalf + j][lane];
-        if (g % 2 == 0) {
+        for (int j = 0; j < kAhead; ++j) w[j] = du[g * kAhead + j][lane];
+        if (g * kAhead % kScanGroup == 0) {
           wait_scalars();
           nowb = nextb;
-          if (g + 2 < kHalves)
-            nextb = load_uniform<u16s>(tile_at(tile, r) + (g / 2 + 1) * 4 * kScanGroup);
+          if (g * kAhead + kScanGroup < kScanTile)
+            nextb = load_uniform<u16s>(tile_at(tile, r) + (g * kAhead + kScanGroup) * 4);
           else
             next = load_half(tile_at(tile, r), kHalves - 1);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < kScanHalf; ++j) {
-          const int t = g * kScanHalf + j;
+        for (int j = 0; j < kAhead; ++j) {
+          const int t = g * kAhead + j;
 #pragma unroll
           for (int i = 0; i < kScanStates; ++i) {
             e[t][i] = __builtin_amdgcn_exp2f(w[j].x * a2[i]);
-            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(nowb, g % 2 * kScanHalf + j, i));
+            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(nowb, t % kScanGroup, i));
           }
         }
-        pin(s[(g + 1) * kScanHalf]);
+        pin(s[(g + 1) * kAhead]);
         __builtin_amdgcn_sched_barrier(0);
       }
       float rb[kScanTile], rc[kScanTile], ga[kScanStates] = {};
