@@ -38,6 +38,8 @@ _TYPES = {torch.float32: _lib.PT_F32, torch.bfloat16: _lib.PT_BF16}
 
 
 # --- argument checks -----------------------------------------------------------
+# A single token's call is host time, of which these checks are a part: they
+# read each attribute once and build nothing that a valid call does not need.
 def _activation(x: torch.Tensor, ndim: int, what: str) -> int:
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
@@ -57,8 +59,9 @@ def _like(t: torch.Tensor, x: torch.Tensor, shape: tuple, name: str) -> None:
 
 def _weights(t: torch.Tensor | None, x: torch.Tensor, shape: tuple, name: str):
     """A float32 parameter of that shape, contiguous; None stays None."""
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.float32 and t.shape == shape and t.device == x.device
+                     and t.is_contiguous()):
+        return t
     if t.dtype != torch.float32 or t.device != x.device or t.shape != shape:
         raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)} on x's device")
     return t.contiguous()
@@ -84,22 +87,28 @@ def _slots(t: torch.Tensor | None, x: torch.Tensor, pool: int):
 
 
 def _pool(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, row: tuple) -> int:
-    if (t.dtype != dtype or t.device != x.device or t.ndim != 3 or t.shape[1:] != row
-            or not t.is_contiguous()):
+    shape = t.shape
+    if not (t.dtype is dtype and len(shape) == 3 and shape[1] == row[0] and shape[2] == row[1]
+            and t.is_contiguous() and t.device == x.device):
         raise ValueError(f"state must be a contiguous {str(dtype)[6:]} tensor of shape "
                          f"{('pool', *row)} on x's device")
-    return t.shape[0]
+    return shape[0]
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with its last dimension contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _near_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` as the scan takes it: rows also less than 2^25 values apart."""
     t = _rows(t)
     return t if t.ndim < 3 or 0 <= t.stride(1) < 1 << 25 else t.contiguous()
+
+
+def _stride(t: torch.Tensor) -> int:
+    """What rows of [rows, H] are apart, in elements; 0 for a single one."""
+    return t.stride()[0] if t.shape[0] > 1 else 0
 
 
 def _strides(t: torch.Tensor, n: int) -> list[int]:
@@ -112,7 +121,11 @@ def _opt(t: torch.Tensor | None):
 
 
 def _asks_gradient(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _bytes(query: str, *args: Any) -> int:
@@ -247,8 +260,9 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
     x = _rows(x)
     y = torch.empty(B, H, dtype=x.dtype, device=x.device)
     if y.numel():
-        _call(_lib.load().pt_causal_conv_step, x.device, kind, _ptr(x), *_strides(x, 1),
-              _ptr(weight), _opt(bias), _ptr(state), _opt(slots), _ptr(y), B, H, K, pool, silu)
+        _call(_lib.load().pt_causal_conv_step, x.device, kind, x.data_ptr(), _stride(x),
+              weight.data_ptr(), _opt(bias), state.data_ptr(), _opt(slots), y.data_ptr(), B, H, K,
+              pool, silu)
     return y
 
 
@@ -401,7 +415,11 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
 # --- the norms -----------------------------------------------------------------
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """[..., H] as [rows, H] with contiguous channels."""
-    return _rows(t if t.ndim == 2 else t.reshape(-1, t.shape[-1]))
+    return _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+
+
+def _shaped(t: torch.Tensor, shape: torch.Size) -> torch.Tensor:
+    return t if len(shape) == 2 else t.view(shape)
 
 
 def _norm_input(x: torch.Tensor) -> int:
@@ -417,8 +435,8 @@ def _gated_forward(x, gate, weight, eps, groups, train):
     rows, H = x.shape
     y = torch.empty(rows, H, dtype=x.dtype, device=x.device)
     rstd = torch.empty(rows * groups, dtype=torch.float32, device=x.device) if train else None
-    _call(_lib.load().pt_gated_norm_fwd, x.device, _TYPES[x.dtype], _ptr(x), *_strides(x, 1),
-          _ptr(gate), *_strides(gate, 1), _ptr(weight), _ptr(y), _opt(rstd), rows, H, groups, eps)
+    _call(_lib.load().pt_gated_norm_fwd, x.device, _TYPES[x.dtype], _ptr(x), _stride(x),
+          _ptr(gate), _stride(gate), _ptr(weight), _ptr(y), _opt(rstd), rows, H, groups, eps)
     return y, rstd
 
 
@@ -440,8 +458,8 @@ class GatedNorm(torch.autograd.Function):
         gx, gg, gw = torch.empty_like(gy), torch.empty_like(gy), torch.empty_like(weight)
         kind = _TYPES[x.dtype]
         ws = _workspace(_bytes("pt_gated_norm_bwd_workspace_bytes", kind, rows, H, ctx.groups), x)
-        _call(_lib.load().pt_gated_norm_bwd, x.device, kind, _ptr(x), *_strides(x, 1), _ptr(gate),
-              *_strides(gate, 1), _ptr(weight), _ptr(rstd), _ptr(gy), _ptr(gx), _ptr(gg), _ptr(gw),
+        _call(_lib.load().pt_gated_norm_bwd, x.device, kind, _ptr(x), _stride(x), _ptr(gate),
+              _stride(gate), _ptr(weight), _ptr(rstd), _ptr(gy), _ptr(gx), _ptr(gg), _ptr(gw),
               _opt(ws), 0 if ws is None else ws.numel(), rows, H, ctx.groups)
         return gx, gg, gw, None, None
 
@@ -459,21 +477,21 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, *, gro
         raise ValueError(f"groups must divide H into parts of at most {MAX_NORM_CHANNELS} channels")
     shape, x, gate = x.shape, _flat(x), _flat(gate)
     if _asks_gradient(x, gate, weight):
-        return GatedNorm.apply(x, gate, weight, float(eps), int(groups)).view(shape)
-    return _gated_forward(x, gate, weight, float(eps), int(groups), False)[0].view(shape)
+        return _shaped(GatedNorm.apply(x, gate, weight, float(eps), int(groups)), shape)
+    return _shaped(_gated_forward(x, gate, weight, float(eps), int(groups), False)[0], shape)
 
 
 def _residual_forward(x, residual, weight, post_weight, scale, eps, train):
     rows, H = x.shape
-    kind = _TYPES[x.dtype]
+    dtype, dev = x.dtype, x.device
     res = x if residual is None else residual
-    y = torch.empty(rows, H, dtype=x.dtype, device=x.device)
-    out = torch.empty(rows, H, dtype=res.dtype, device=x.device)
+    y = torch.empty(rows, H, dtype=dtype, device=dev)
+    out = torch.empty(rows, H, dtype=res.dtype, device=dev)
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if train else None
     rstd_x = torch.empty_like(rstd) if train and post_weight is not None else None
-    _call(_lib.load().pt_residual_norm_fwd, x.device, kind, _TYPES[res.dtype], _ptr(x),
-          *_strides(x, 1), _opt(residual), *_strides(res, 1), _opt(post_weight), _opt(scale),
-          _ptr(weight), _ptr(y), _ptr(out), _opt(rstd), _opt(rstd_x), rows, H, eps)
+    _call(_lib.load().pt_residual_norm_fwd, dev, _TYPES[dtype], _TYPES[res.dtype], x.data_ptr(),
+          _stride(x), _opt(residual), _stride(res), _opt(post_weight), _opt(scale),
+          weight.data_ptr(), y.data_ptr(), out.data_ptr(), _opt(rstd), _opt(rstd_x), rows, H, eps)
     return y, out, rstd, rstd_x
 
 
@@ -504,7 +522,7 @@ class ResidualNorm(torch.autograd.Function):
         kind = _TYPES[x.dtype]
         ws = _workspace(_bytes("pt_residual_norm_bwd_workspace_bytes", kind, rows, H, sums), x)
         _call(_lib.load().pt_residual_norm_bwd, x.device, kind, _TYPES[ctx.out_type], _ptr(x),
-              *_strides(x, 1), _opt(residual), *_strides(x if residual is None else residual, 1),
+              _stride(x), _opt(residual), _stride(x if residual is None else residual),
               _opt(post_weight), _opt(scale), _ptr(weight), _ptr(rstd), _opt(rstd_x), _ptr(gy),
               _opt(gout), _ptr(gx), _opt(gres), _ptr(params), _opt(ws),
               0 if ws is None else ws.numel(), rows, H)
@@ -543,7 +561,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.
         y, out = ResidualNorm.apply(x, residual, weight, post_weight, scale, float(eps))
     else:
         y, out, _, _ = _residual_forward(x, residual, weight, post_weight, scale, float(eps), False)
-    return y.view(shape), out.view(shape)
+    return _shaped(y, shape), _shaped(out, shape)
 
 
 __all__ = [
