@@ -393,8 +393,8 @@ int pt_s4_head_grad_f32(const float* x, const float* gy, const float* w, float* 
  * that a slice of a projection's output can be passed as it is. Outputs are
  * contiguous. Pointers need their type's alignment; 16-byte aligned ones with
  * strides and channels in multiples of 16 bytes take wide loads. Offsets are
- * 64-bit: only each size is limited (PT_ERR_SHAPE), and a launch to 2^32
- * lanes. B (or rows) = 0 launches nothing but zero parameter gradients.
+ * 64-bit: only each size is limited (PT_ERR_SHAPE; L to 2^30), and a launch
+ * to 2^32 lanes. B (or rows) = 0 launches nothing but zero parameter gradients.
  * Parameter gradients are added in a fixed order. `lengths` [B] (NULL: all L)
  * are the tokens of each sequence, clamped to [0, L]; what lies past them is
  * not used, and outputs and gradients there are 0.

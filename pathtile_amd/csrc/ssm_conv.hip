@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kSumThreads) void causal_reduce_kernel(const float*
 
 static int check_causal(int dtype, int B, int L, int H, int K) {
   if (dtype != PT_F32 && dtype != PT_BF16) return PT_ERR_CONFIG;
-  if (B < 0 || L < 1 || H < 1 || K < 1 || K > kCausalMaxK) return PT_ERR_SHAPE;
+  if (B < 0 || L < 1 || L > kCausalMaxL || H < 1 || K < 1 || K > kCausalMaxK) return PT_ERR_SHAPE;
   return PT_OK;
 }
 

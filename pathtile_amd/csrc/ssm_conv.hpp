@@ -20,6 +20,7 @@
 namespace pt {
 
 constexpr int kCausalMaxK = 8;
+constexpr int kCausalMaxL = 1 << 30;  // a step past the end still counts its tokens in int
 constexpr int kCausalThreads = 256;
 constexpr int kCausalFwdStep = 4, kCausalBwdStep = 4;  // tokens at a time; a run is a multiple
 

@@ -30,7 +30,7 @@ __global__ __launch_bounds__(kSumThreads) void scan_param_reduce_kernel(
 
 static int check_scan(const pt_scan_inputs* in, int L) {
   if (in->dtype != PT_F32 && in->dtype != PT_BF16) return PT_ERR_CONFIG;
-  if (in->B < 0 || L < 1 || in->H < 1 || in->N < 1 || in->N > kScanMaxN || in->G < 1 || in->H % in->G)
+  if (in->B < 0 || L < 1 || L > kScanMaxL || in->H < 1 || in->N < 1 || in->N > kScanMaxN || in->G < 1 || in->H % in->G)
     return PT_ERR_SHAPE;
   if (in->b_group < 0 || in->c_group < 0 || in->b_group >= (1LL << 31) || in->c_group >= (1LL << 31))
     return PT_ERR_SHAPE;
@@ -46,7 +46,7 @@ static int check_scan(const pt_scan_inputs* in, int L) {
 // chunks 225 and 160); fewer are cut into chunks of four tiles or more, two to
 // each of 256 CUs, which costs the pass for their states.
 static int scan_chunk_tiles(long long blocks, int ntiles) {
-  long long chunks = blocks >= 160 ? 1 : ssm_ceil(512, blocks);
+  long long chunks = blocks < 1 || blocks >= 160 ? 1 : ssm_ceil(512, blocks);
   if (chunks > ntiles / 4) chunks = ntiles / 4;
   return (int)ssm_ceil(ntiles, chunks > 1 ? chunks : 1);
 }

@@ -27,6 +27,7 @@ constexpr int kScanStates = 2;     // of a wave: 16 a round
 constexpr int kScanThreads = 512;
 constexpr int kScanCols = 2;       // channels of a token that a thread loads and stores
 constexpr int kScanMaxN = 64;
+constexpr int kScanMaxL = 1 << 30;  // a tile past the end still counts its tokens in int
 
 struct ScanArgs {
   const void *x, *dt;           // [B, L, H]

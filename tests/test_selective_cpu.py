@@ -32,7 +32,7 @@ def test_scan_refusals(lib):
     def fwd(**kw):
         return lib.pt_selective_scan_fwd(ctypes.byref(_scan(**kw)), 4096, None, None, None, 0, None)
 
-    for kw in ({"L": 0}, {"H": 0}, {"N": 0}, {"N": 65}, {"G": 0}, {"G": 3}, {"B": -1},
+    for kw in ({"L": 0}, {"L": (1 << 30) + 1}, {"H": 0}, {"N": 0}, {"N": 65}, {"G": 0}, {"G": 3}, {"B": -1},
                {"b_group": -1}, {"b_group": 2**31}):
         assert fwd(**kw) == _lib.PT_ERR_SHAPE, kw
     assert fwd(dtype=2) == _lib.PT_ERR_CONFIG
@@ -65,6 +65,7 @@ def test_scan_sizes(lib):
     assert bwd >= B * L * 2 * 16 * 4
     assert sizes(B=B, L=L, H=H, N=13) == [ws, saved, bwd]
     assert sizes(B=B, L=L, H=H, N=17)[1] > saved
+    assert sizes(B=0)[1:] == [0, 0]
     # 64-bit sizes
     big = sizes(B=64, L=1 << 20, H=4096, N=64)
     assert big[1] > 64 * (1 << 16) * 64 * 4096 * 4
@@ -77,7 +78,7 @@ def test_conv_refusals(lib):
         return lib.pt_causal_conv_fwd(dtype, x, L * H, H, 4096, None, None, None, 4096, None,
                                       B, L, H, K, 1, None)
 
-    for kw in ({"B": -1}, {"L": 0}, {"H": 0}, {"K": 0}, {"K": 9}):
+    for kw in ({"B": -1}, {"L": 0}, {"L": (1 << 30) + 1}, {"H": 0}, {"K": 0}, {"K": 9}):
         assert fwd(**kw) == _lib.PT_ERR_SHAPE, kw
     assert fwd(dtype=7) == _lib.PT_ERR_CONFIG
     assert fwd(x=None) == _lib.PT_ERR_NULL
