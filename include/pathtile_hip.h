@@ -392,9 +392,10 @@ int pt_s4_head_grad_f32(const float* x, const float* gy, const float* w, float* 
  * FP32. Rows hold contiguous channels; strides of inputs are in elements, so
  * that a slice of a projection's output can be passed as it is. Outputs are
  * contiguous. Pointers need their type's alignment; 16-byte aligned ones with
- * strides and channels in multiples of 16 bytes take wide loads. Offsets are
- * 64-bit: only each size is limited (PT_ERR_SHAPE; L to 2^30), and a launch
- * to 2^32 lanes. B (or rows) = 0 launches nothing but zero parameter gradients.
+ * strides and channels in multiples of 16 bytes take wide loads. Workspaces of
+ * the convolution's backward are 16-byte aligned, those of the scan and `saved`
+ * 64-byte (PT_ERR_ALIGN). Offsets are 64-bit: only each size is limited
+ * (PT_ERR_SHAPE; L to 2^30), and a launch to 2^32 lanes. B (or rows) = 0 launches nothing but zero parameter gradients.
  * Parameter gradients are added in a fixed order. `lengths` [B] (NULL: all L)
  * are the tokens of each sequence, clamped to [0, L]; what lies past them is
  * not used, and outputs and gradients there are 0.
@@ -440,8 +441,8 @@ int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* 
  * groups); A [H, N]; D and dt_bias [H] or NULL (0); the first state [B, H, N]
  * or NULL (0). H and the row strides of x and dt are below 2^25.
  * _sizes gives the bytes of the workspaces and of `saved`, which _fwd fills
- * where not NULL (the state before every 16 tokens) and _bwd takes with the
- * same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;
+ * where not NULL (the state before every 16 tokens, and B and C in the order
+ * that the kernels read) and _bwd takes with the same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;
  * gd, gdt_bias and gstate are skipped where NULL; gb, gc are [B, L, G, N].
  * _step: one token, x and dt [B, H] and B, C [B, G, N] with the batch strides
  * (row strides and L are not read); states [pool, H, N] and slots as in

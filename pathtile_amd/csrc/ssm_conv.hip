@@ -128,6 +128,7 @@ int pt_causal_conv_bwd(int dtype, const void* x, long long x_batch, long long x_
   if (B > 0) {
     if (!x || !w || !gy || !gx) return PT_ERR_NULL;
     if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
+    if (!pt::ssm_aligned(workspace, 16)) return PT_ERR_ALIGN;  // sums are stored by fours
   }
   const void* ptrs[] = {x, state, gy, gstate_out, gx, gstate};
   const int v = pt::causal_lanes(dtype, 4, H, x_batch, x_row, ptrs, 6);

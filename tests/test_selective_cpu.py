@@ -150,3 +150,15 @@ def test_model_parameters_and_cache():
     cache.scan[0] += 1
     cache.clear(torch.tensor([2]))
     assert cache.scan[0][0].all() and not cache.scan[0][2].any()
+
+
+def test_workspaces_are_aligned(lib):
+    """Workspaces that are read and written by vectors are refused at odd addresses."""
+    from pathtile_amd import _lib
+
+    conv = [0, 4096, 40, 8] + [4096] * 10
+    assert lib.pt_causal_conv_bwd(*conv, 4100, 1 << 20, 2, 5, 8, 4, 1, None) == _lib.PT_ERR_ALIGN
+    s = ctypes.byref(_scan())
+    assert lib.pt_selective_scan_fwd(s, 4096, None, None, 4112, 1 << 20, None) == _lib.PT_ERR_ALIGN
+    assert lib.pt_selective_scan_fwd(s, 4096, None, 4112, 4096, 1 << 20, None) == _lib.PT_ERR_ALIGN
+    assert lib.pt_selective_scan_bwd(s, *[4096] * 11, 4112, 1 << 20, None) == _lib.PT_ERR_ALIGN
