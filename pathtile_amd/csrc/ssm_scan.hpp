@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
   const bool mine = lane < p.nh;
   const int h = p.h0 + lane;
   Rounds<MANY> states(hold);
-  float a2[kScanStates], steps = 0.0f;
+  float a2[kScanStates], steps[kScanCols] = {};
   const float zero[kScanStates] = {};
   for (int r = 0; r < rounds; ++r) states.set(r, zero);
   load_rates(a, mine, h, 0, wave, a2);
@@ -369,6 +369,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
     for (int i = 0; i < kScanCols; ++i) {
       const float x = at_few(xv, i), z = in ? d[i] : 0.0f;  // past the end nothing changes
       du[tile & 1][row][c0 + i] = make_float2(z, REV ? x : z * x);
+      steps[i] += z;
     }
   };
   const int tiles = (len + kScanTile - 1) / kScanTile;
@@ -427,16 +428,17 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
         for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
       }
     }
-    float sum = 0.0f;
-#pragma unroll
-    for (int t = 0; t < kScanTile; ++t) sum += q[t].x;
-    steps += sum;
     if (k + 1 < n) {
       put(at(k + 1));
       if (k + 2 < n) fetch(at(k + 2));
     }
     __syncthreads();
   }
+  // The sums of the steps are by tokens of a tile's rows.
+  float* sums = &du[0][0][0].x;
+#pragma unroll
+  for (int i = 0; i < kScanCols; ++i) sums[row * kScanCh + c0 + i] = steps[i];
+  __syncthreads();
   if (!mine) return;
   const long long out = (long long)p.b * a.chunks + p.c;
   for (int r = 0; r < rounds; ++r) {
@@ -445,7 +447,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
 #pragma unroll
     for (int i = 0; i < kScanStates; ++i) f.states[state_at(a, out, r, wave, h) + (long long)i * a.H] = s[i];
   }
-  if (wave == 0) f.steps[out * a.H + h] = steps;
+  if (wave == 0) {
+    float sum = 0.0f;
+    for (int t = 0; t < kScanTile; ++t) sum += sums[t * kScanCh + lane];
+    f.steps[out * a.H + h] = sum;
+  }
 }
 
 struct ScanFwdArgs {
