@@ -171,9 +171,25 @@ __device__ __forceinline__ void store_few(T* p, int n, const float (&v)[V]) {
 // offset in bytes, below 2^31 within a tile.
 template <typename T>
 __device__ __forceinline__ T* lane_at(T* base, uint32_t bytes) {
-  return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + bytes);
+  return reinterpret_cast<T*>((char*)base + bytes);
 }
 constexpr long long kScanMaxRow = 1LL << 25;  // values: 16 rows of FP32 are 2^31 bytes
+
+// A thread's channels of a tile's row `row`; `p` is the tile's first row, the
+// first `rows` >= 1 of which are there. By vectors the load has no condition
+// and so nothing to wait for: a row or channel that is not there is another,
+// which the caller leaves out.
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void fetch_row(const T* p, long long stride, int row, int rows, int c0, int cn,
+                                          Few<T, V, VEC>& f) {
+  if constexpr (VEC) {
+    const uint32_t at = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)stride + (cn > 0 ? c0 : 0);
+    f.v = *reinterpret_cast<const decltype(f.v)*>(lane_at(p, at * (uint32_t)sizeof(T)));
+  } else {
+    f = {};
+    if (row < rows) fetch_few(lane_at(p, ((uint32_t)row * (uint32_t)stride + c0) * (uint32_t)sizeof(T)), cn, f);
+  }
+}
 
 // B and C into that layout, one token and two states a thread.
 template <typename T>
@@ -230,7 +246,11 @@ __device__ __forceinline__ void load_states(const float* p, bool mine, const Sca
 #pragma unroll
   for (int i = 0; i < kScanStates; ++i) {
     const int n = (r * kScanWaves + wave) * kScanStates + i;
-    v[i] = p && mine && n < a.N ? p[row * a.N + n] : 0.0f;
+    v[i] = 0.0f;
+    if (p) {  // a lane without a channel and a state past N read another value
+      const float q = p[row * a.N + (n < a.N ? n : 0)];
+      v[i] = mine && n < a.N ? q : 0.0f;
+    }
   }
 }
 __device__ __forceinline__ void store_states(float* p, bool mine, const ScanArgs& a, long long row,
@@ -324,19 +344,25 @@ template <typename T, bool MANY, bool VEC, bool REV>
 __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs f) {
   constexpr int kGroups = kScanTile / kScanGroup;
   __shared__ float2 du[2][kScanTile][kScanCh];
-  __shared__ typename Rounds<MANY>::Lds hold;
+  __shared__ typename Rounds<MANY>::Lds hold, hold_a2;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
   if (p.c == (REV ? 0 : a.chunks - 1)) return;  // no chunk starts from its state
   const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
-  const int h = p.h0 + lane;
-  Rounds<MANY> states(hold);
-  float a2[kScanStates], steps[kScanCols] = {};
+  const int h = p.h0 + (mine ? lane : 0);
+  Rounds<MANY> states(hold), rates(hold_a2);
+  float steps[kScanCols] = {};
   const float zero[kScanStates] = {};
-  for (int r = 0; r < rounds; ++r) states.set(r, zero);
-  load_rates(a, mine, h, 0, wave, a2);
+#pragma unroll
+  for (int r = 0; r < (MANY ? kScanRounds : 1); ++r) {
+    if (r >= rounds) break;
+    float a2[kScanStates];
+    load_rates(a, mine, h, r, wave, a2);
+    rates.set(r, a2);
+    states.set(r, zero);
+  }
 
   const int row = tid >> 5, c0 = (tid & 31) * kScanCols, cn = p.nh - c0;
   const long long xrow = REV ? a.H : a.x_row;
@@ -396,9 +422,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
     for (int t = 0; t < kScanTile; ++t) q[t] = du[tile & 1][t][lane];
     for (int r = 0; r < rounds; ++r) {
       const bool more = r + 1 < rounds;
-      float s[kScanStates], a3[kScanStates];
+      float s[kScanStates], a2[kScanStates];
       states.get(r, s);
-      if (MANY) load_rates(a, mine, h, more ? r + 1 : 0, wave, a3);
+      rates.get(r, a2);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         wait_scalars();
@@ -423,10 +449,6 @@ __global__ __launch_bounds__(kScanThreads) void scan_chunk_kernel(ScanChunkArgs 
         __builtin_amdgcn_sched_barrier(0);
       }
       states.set(r, s);
-      if (MANY) {
-#pragma unroll
-        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
-      }
     }
     if (k + 1 < n) {
       put(at(k + 1));
@@ -469,20 +491,22 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
   __shared__ float2 du[2][kScanTile][kScanCh];
   // Many rounds: one buffer and a second barrier, and so two workgroups a CU.
   __shared__ float yp[MANY ? 1 : 2][kScanWaves][kScanTile][kScanCh];
-  __shared__ typename Rounds<MANY>::Lds hold;
+  __shared__ typename Rounds<MANY>::Lds hold, hold_a2;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
   const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
-  const int h = p.h0 + lane;
+  const int h = p.h0 + (mine ? lane : 0);
   const uint32_t ho = (uint32_t)h * sizeof(float);
 
-  Rounds<MANY> states(hold);
-  float a2[kScanStates];
-  for (int r = rounds - 1; r >= 0; --r) {
-    float s[kScanStates];
-    if (r == 0 || p.c > 0) load_rates(a, mine, h, r, wave, a2);
+  Rounds<MANY> states(hold), rates(hold_a2);
+#pragma unroll
+  for (int r = 0; r < (MANY ? kScanRounds : 1); ++r) {
+    if (r >= rounds) break;
+    float s[kScanStates], a2[kScanStates];
+    load_rates(a, mine, h, r, wave, a2);
+    rates.set(r, a2);
     load_states(a.state, mine, a, (long long)p.b * a.H + h, r, wave, s);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, 0, p.c, r, wave, h, a2, s);
     states.set(r, s);
@@ -549,9 +573,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
     for (int t = 0; t < kScanTile; ++t) q[t] = du[buf][t][lane], y[t] = 0.0f;
     for (int r = 0; r < rounds; ++r) {
       const bool more = r + 1 < rounds;
-      float s[kScanStates], a3[kScanStates];
+      float s[kScanStates], a2[kScanStates];
       states.get(r, s);
-      if (MANY) load_rates(a, mine, h, more ? r + 1 : 0, wave, a3);
+      rates.get(r, a2);
       if (f.saved && mine) {
         float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, 0);
 #pragma unroll
@@ -579,10 +603,6 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
         __builtin_amdgcn_sched_barrier(0);
       }
       states.set(r, s);
-      if (MANY) {
-#pragma unroll
-        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
-      }
     }
 #pragma unroll
     for (int t = 0; t < kScanTile; ++t) yp[MANY ? 0 : buf][wave][t][lane] = y[t];
@@ -665,35 +685,40 @@ __device__ __forceinline__ float fold_row(float u, float v, bool bit) {
 constexpr int kDppRor8 = 0x128, kDppHalfMirror = 0x141, kDppXor2 = 0x4e, kDppXor1 = 0xb1;
 
 template <typename T, bool MANY, bool VEC>
-__global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(ScanBwdArgs f) {
+__global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f) {
   constexpr int kHalves = kScanTile / kScanHalf;
-  constexpr int kAhead = MANY ? kScanGroup : kScanHalf;  // tokens asked of LDS at a time
   __shared__ float2 du[kScanTile][kScanCh];
   __shared__ float gys[kScanTile][kScanCh];
   __shared__ float p1[kScanWaves][kScanTile][kScanCh], p2[kScanWaves][kScanTile][kScanCh];
   __shared__ float bias[kScanCh], dskip[kScanCh];
-  __shared__ typename Rounds<MANY>::Lds hold_q, hold_a;
+  __shared__ typename Rounds<MANY>::Lds hold_q, hold_a, hold_a2;
   const ScanArgs& a = f.s;
   const ScanPlace p = scan_place(a, blockIdx.x);
   const int len = scan_length(a, p.b), rounds = scan_rounds<MANY>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool mine = lane < p.nh;
-  const int h = p.h0 + lane;
+  const int h = p.h0 + (mine ? lane : 0);
   const uint32_t ho = (uint32_t)h * sizeof(float);
   const int tiles = (len + kScanTile - 1) / kScanTile;
   const int last = p.last < tiles ? p.last : tiles;
 
-  Rounds<MANY> qs(hold_q), gas(hold_a);
+  Rounds<MANY> qs(hold_q), gas(hold_a), rates(hold_a2);
   const float zero[kScanStates] = {};
-  float a2[kScanStates], s0[kScanStates];  // of the round at hand
+  float s0[kScanStates];  // of the round at hand
   auto load_saved = [&](int tile, int r, float(&v)[kScanStates]) {
     const float* sp = f.saved + state_at(a, (long long)p.b * a.ntiles + tile, r, wave, 0);
 #pragma unroll
-    for (int i = 0; i < kScanStates; ++i) v[i] = mine ? *lane_at(sp + (long long)i * a.H, ho) : 0.0f;
+    for (int i = 0; i < kScanStates; ++i) {
+      const float q = *lane_at(sp + (long long)i * a.H, ho);
+      v[i] = mine ? q : 0.0f;
+    }
   };
-  for (int r = rounds - 1; r >= 0; --r) {
-    float q[kScanStates];
-    if (r == 0 || p.c < a.chunks - 1) load_rates(a, mine, h, r, wave, a2);
+#pragma unroll
+  for (int r = 0; r < (MANY ? kScanRounds : 1); ++r) {
+    if (r >= rounds) break;
+    float q[kScanStates], a2[kScanStates];
+    load_rates(a, mine, h, r, wave, a2);
+    rates.set(r, a2);
     load_states(f.gstate_out, mine, a, (long long)p.b * a.H + h, r, wave, q);
     if (mine) join_chunks(a, f.chunk_states, f.chunk_steps, p.b, a.chunks - 1, p.c, r, wave, h, a2, q);
     qs.set(r, q);
@@ -708,7 +733,6 @@ __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(Sc
   T* gxp = static_cast<T*>(f.gx) + yb;
   T* gdp = static_cast<T*>(f.gdt) + yb;
   float* pp = f.part_bc + ((long long)p.blk * a.B + p.b) * a.L * 2 * a.np;
-  const uint32_t xo = (uint32_t)(row * a.x_row + c0) * sizeof(T), dto = (uint32_t)(row * a.dt_row + c0) * sizeof(T);
   const uint32_t oo = (uint32_t)(row * a.H + c0) * sizeof(T);
   // What the folds leave in a lane: state lane / 32, token of bits 4, 3, 2, 1, B
   // or C.
@@ -727,89 +751,114 @@ __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(Sc
   }
   Few<T, kScanCols, VEC> xv, dv, gv;
   auto fetch = [&](int tile) {
-    xv = {}, dv = {}, gv = {};
-    if (tile * kScanTile + row < len && cn > 0) {
-      fetch_few(lane_at(xp + (long long)tile * kScanTile * a.x_row, xo), cn, xv);
-      fetch_few(lane_at(dp + (long long)tile * kScanTile * a.dt_row, dto), cn, dv);
-      fetch_few(lane_at(gp + (long long)tile * kScanTile * a.H, oo), cn, gv);
-    }
+    const int t = tile * kScanTile;
+    fetch_row(xp + t * a.x_row, a.x_row, row, len - t, c0, cn, xv);
+    fetch_row(dp + t * a.dt_row, a.dt_row, row, len - t, c0, cn, dv);
+    fetch_row(gp + (long long)t * a.H, a.H, row, len - t, c0, cn, gv);
   };
   const size_t pair = (size_t)a.ntiles * kScanTile * 4;  // floats of two states
   const float* bc = f.bc + ((size_t)(p.b * a.G + p.g) * (a.np / 2) + wave) * pair;
   auto tile_at = [&](int tile, int r) { return bc + r * kScanWaves * pair + (size_t)tile * kScanTile * 4; };
   BcHalf next;
-  u16s nextb = {}, nowb;
+  u16s nextb = {};
   if (p.first < last) {
     nextb = load_uniform<u16s>(tile_at(last - 1, 0));
     fetch(last - 1);
     load_saved(last - 1, 0, s0);
   }
+  // A tile's d, d x and gy: in registers, then in LDS.
+  float xk[kScanCols], sg[kScanCols], x[kScanCols], gy[kScanCols], d[kScanCols], grad[kScanCols];
+  auto steps = [&](int tile) {
+    const bool in = tile * kScanTile + row < len && cn > 0;
+#pragma unroll
+    for (int i = 0; i < kScanCols; ++i) {
+      // 0 past the end and where there is no channel: these go into the sums
+      x[i] = in ? at_few(xv, i) : 0.0f, gy[i] = in ? at_few(gv, i) : 0.0f;
+      d[i] = at_few(dv, i) + bias[c0 + i], grad[i] = 1.0f;
+    }
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &grad[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kScanCols; ++i) d[i] = in ? d[i] : 0.0f;  // past the end nothing changes
+  };
+  auto put = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < kScanCols; ++i) {
+      xk[i] = x[i], sg[i] = grad[i];
+      du[row][c0 + i] = make_float2(d[i], d[i] * x[i]);
+      gys[row][c0 + i] = gy[i];
+    }
+    if (tile > p.first) fetch(tile - 1);
+  };
   wait_loads();
+  __syncthreads();
+  if (p.first < last) steps(last - 1), put(last - 1);
   __syncthreads();
   for (int tile = last - 1; tile >= p.first; --tile) {
     const int t0 = tile * kScanTile;
     const bool in = t0 + row < len;
-    float d[kScanCols], sg[kScanCols];
-    const Few<T, kScanCols, VEC> xk = xv;
-#pragma unroll
-    for (int i = 0; i < kScanCols; ++i) d[i] = at_few(dv, i) + bias[c0 + i], sg[i] = 1.0f;
-    if (a.softplus) {
-#pragma unroll
-      for (int i = 0; i < kScanCols; ++i) d[i] = softplus_f32(d[i], &sg[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kScanCols; ++i) {
-      d[i] = in ? d[i] : 0.0f;  // past the end nothing changes
-      du[row][c0 + i] = make_float2(d[i], d[i] * at_few(xk, i));
-      gys[row][c0 + i] = at_few(gv, i);
-    }
-    if (tile > p.first) fetch(tile - 1);
-    __syncthreads();
     float s1[kScanTile], s2[kScanTile];  // sums over a wave's states
     for (int r = 0; r < rounds; ++r) {
-      float s[kScanTile + 1][kScanStates], e[kScanTile][kScanStates], q[kScanStates], a3[kScanStates];
+      float s[kScanTile + 1][kScanStates], e[kScanTile][kScanStates], q[kScanStates], a2[kScanStates];
       const bool more = r + 1 < rounds;
       const int tile2 = more || tile == p.first ? tile : tile - 1, r2 = more ? r + 1 : 0;
 #pragma unroll
       for (int i = 0; i < kScanStates; ++i) s[0][i] = s0[i];
       load_saved(tile2, r2, s0);
-      if (MANY) load_rates(a, mine, h, r2, wave, a3);
+      rates.get(r, a2);
       // Forward with B alone, then back with both.
+      float2 wf[kScanGroup];
 #pragma unroll
-      for (int g = 0; g < kScanTile / kAhead; ++g) {
-        float2 w[kAhead];
+      for (int j = 0; j < kScanGroup; ++j) wf[j] = du[j][lane];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) w[j] = du[g * kAhead + j][lane];
-        if (g * kAhead % kScanGroup == 0) {
-          wait_scalars();
-          nowb = nextb;
-          if (g * kAhead + kScanGroup < kScanTile)
-            nextb = load_uniform<u16s>(tile_at(tile, r) + (g * kAhead + kScanGroup) * 4);
-          else
-            next = load_half(tile_at(tile, r), kHalves - 1);
+      for (int g = 0; g < kScanTile / kScanGroup; ++g) {
+        float2 w[kScanGroup];
+        wait_scalars();
+#pragma unroll
+        for (int j = 0; j < kScanGroup; ++j) w[j] = wf[j];
+        if (g + 1 < kScanTile / kScanGroup) {
+#pragma unroll
+          for (int j = 0; j < kScanGroup; ++j) wf[j] = du[(g + 1) * kScanGroup + j][lane];
         }
+        const u16s nowb = nextb;
+        if (g + 1 < kScanTile / kScanGroup)
+          nextb = load_uniform<u16s>(tile_at(tile, r) + (g + 1) * kScanGroup * 4);
+        else
+          next = load_half(tile_at(tile, r), kHalves - 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int t = g * kAhead + j;
+        for (int j = 0; j < kScanGroup; ++j) {
+          const int t = g * kScanGroup + j;
 #pragma unroll
           for (int i = 0; i < kScanStates; ++i) {
             e[t][i] = __builtin_amdgcn_exp2f(w[j].x * a2[i]);
-            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(nowb, t % kScanGroup, i));
+            s[t + 1][i] = fmaf(e[t][i], s[t][i], w[j].y * uniform_at(nowb, j, i));
           }
         }
-        pin(s[(g + 1) * kAhead]);
+        pin(s[(g + 1) * kScanGroup]);
         __builtin_amdgcn_sched_barrier(0);
       }
       float rb[kScanTile], rc[kScanTile], ga[kScanStates] = {};
       qs.get(r, q);
+      float2 wn[kScanHalf];
+      float gn[kScanHalf];
+#pragma unroll
+      for (int j = 0; j < kScanHalf; ++j)
+        wn[j] = du[(kHalves - 1) * kScanHalf + j][lane], gn[j] = gys[(kHalves - 1) * kScanHalf + j][lane];
 #pragma unroll
       for (int g = kHalves - 1; g >= 0; --g) {
         float2 w[kScanHalf];
         float gyt[kScanHalf];
-#pragma unroll
-        for (int j = 0; j < kScanHalf; ++j) w[j] = du[g * kScanHalf + j][lane], gyt[j] = gys[g * kScanHalf + j][lane];
         wait_scalars();
+#pragma unroll
+        for (int j = 0; j < kScanHalf; ++j) w[j] = wn[j], gyt[j] = gn[j];
+        if (g > 0) {
+#pragma unroll
+          for (int j = 0; j < kScanHalf; ++j)
+            wn[j] = du[(g - 1) * kScanHalf + j][lane], gn[j] = gys[(g - 1) * kScanHalf + j][lane];
+        }
         const BcHalf now = next;
         if (g > 0)
           next = load_half(tile_at(tile, r), g - 1);
@@ -860,24 +909,38 @@ __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(Sc
       rb[0] = fold_row<kDppXor2>(rb[0], rb[8], lane & 2);
       rc[0] = fold_row<kDppXor2>(rc[0], rc[8], lane & 2);
       rb[0] = fold_row<kDppXor1>(rb[0], rc[0], lane & 1);
+      // Before the stores: a wait for a load is one for the stores before it.
+      if (!more) {
+        if (tile > p.first) {
+          steps(tile - 1);
+          pin(d);
+          pin(grad);
+          pin(x);
+          pin(gy);
+        }
+      }
+      pin(s0);
       if (t0 + pt < len)
         *lane_at(pp + (long long)t0 * 2 * a.np + (r * kScanWaves + wave) * kScanStates, po) = rb[0];
-      if (MANY) {
-#pragma unroll
-        for (int i = 0; i < kScanStates; ++i) a2[i] = a3[i];
-      }
     }
     __syncthreads();
+    float2 g1 = {0.0f, 0.0f}, g2 = g1;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+      const float2 u = *reinterpret_cast<const float2*>(&p1[w][row][c0]);
+      const float2 v = *reinterpret_cast<const float2*>(&p2[w][row][c0]);
+      g1.x += u.x, g1.y += u.y, g2.x += v.x, g2.y += v.y;
+    }
     if (t0 + row < a.L) {
       float ox[kScanCols], od[kScanCols];
 #pragma unroll
       for (int i = 0; i < kScanCols; ++i) {
-        float g1 = 0.0f, g2 = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kScanWaves; ++w) g1 += p1[w][row][c0 + i], g2 += p2[w][row][c0 + i];
-        const float x = at_few(xk, i), gy = gys[row][c0 + i];  // 0 past the end
-        ox[i] = in ? fmaf(du[row][c0 + i].x, g1, dskip[c0 + i] * gy) : 0.0f;
-        od[i] = in ? fmaf(x, g1, kLn2 * g2) * sg[i] : 0.0f;
+        const float x = xk[i], gy = gys[row][c0 + i];  // 0 past the end
+        const float s1 = i ? g1.y : g1.x, s2 = i ? g2.y : g2.x;
+        ox[i] = fmaf(du[row][c0 + i].x, s1, dskip[c0 + i] * gy);
+        od[i] = fmaf(x, s1, kLn2 * s2) * sg[i];
+        ox[i] = in ? ox[i] : 0.0f;
+        od[i] = in ? od[i] : 0.0f;
         gd[i] = fmaf(gy, x, gd[i]);
         gbias[i] += od[i];
       }
@@ -885,6 +948,7 @@ __global__ __launch_bounds__(kScanThreads, MANY ? 2 : 4) void scan_bwd_kernel(Sc
       store_few<VEC, kScanCols>(lane_at(gxp + at, oo), cn, ox);
       store_few<VEC, kScanCols>(lane_at(gdp + at, oo), cn, od);
     }
+    if (tile > p.first) put(tile - 1);  // a thread writes where it alone has read
     __syncthreads();
   }
   const long long part = (long long)p.b * a.chunks + p.c;
