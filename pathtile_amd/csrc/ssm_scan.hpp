@@ -9,10 +9,26 @@
 // A workgroup owns 64 channels of one sequence, a lane each; its eight waves
 // share the channels and split 16 states by twos, so that B and C are the same
 // for all lanes of a wave and come through the scalar cache. More than 16
-// states take rounds of 16 over each tile, with the states of the other rounds
-// in LDS (MANY). Tokens go by tiles of 16: every thread loads two channels of
-// one token and puts d and d x into LDS, the waves run the recurrence on them,
-// and the same threads add the eight waves' parts of y.
+// states take rounds of 16 over each tile, with the states and rates of the
+// other rounds in LDS (MANY). Tokens go by tiles of 16: every thread loads two
+// channels of one token and puts d and d x into LDS, the waves run the recurrence
+// on them, and the same threads add the eight waves' parts of y.
+//
+// Bound by the vector units: a state's step is six issue slots (an exp2 counts
+// for two) for 6 / N bytes of HBM. Two states of one channel a lane leave no
+// product between lanes, so there is nothing for the matrix cores but the sums
+// over channels in the backward, whose results they would give for one lane in
+// 16. In BF16 with 16 states:
+//   1 x 16384 x 2048   first pass 121 us, forward 170 (VALU busy 74 and 76%)
+//   8 x 2048 x 2048    forward 197 us, backward 459 (65 and 75%)
+// where six slots in one pass are 82 us. FP32 2048 x 48 x 128 with 64 states:
+// forward 218 us, backward 656 (72 and 69%).
+// What was measured against it: four waves of four states, 848 us for 670 in
+// both directions of the second size; B and C from other lanes' registers by
+// DPP, 199 us for 171 forward at the first, since such operands issue at half
+// rate; a wave by itself with all 16 states and no LDS, 195 us for 170 there,
+// most of it the joining of its four times as many chunks, and no gain
+// elsewhere.
 
 #pragma once
 
@@ -168,7 +184,9 @@ __device__ __forceinline__ void store_few(T* p, int n, const float (&v)[V]) {
 }
 
 // Addresses are a base that all lanes share, in scalar registers, and a lane's
-// offset in bytes, below 2^31 within a tile.
+// offset in bytes, below 2^31 within a tile. Sums of pointers, not of integers:
+// those would lose the address space, and a load that may be one from LDS is
+// waited for with those.
 template <typename T>
 __device__ __forceinline__ T* lane_at(T* base, uint32_t bytes) {
   return reinterpret_cast<T*>((char*)base + bytes);
@@ -191,7 +209,8 @@ __device__ __forceinline__ void fetch_row(const T* p, long long stride, int row,
   }
 }
 
-// B and C into that layout, one token and two states a thread.
+// B and C into that layout, one token and two states a thread: 4.8 us for the
+// 4 MB of 16384 x 16 x 2, most of it the launch.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(ScanArgs a, float* __restrict__ out) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -331,6 +350,9 @@ __device__ __forceinline__ void join_chunks(const ScanArgs& a, const float* stat
 //   S_c = exp(A D_{c-1}) S_{c-1} + s_{c-1},  S_0 the first state.
 // REV is the same for the backward's q, from the last chunk to the first:
 //   q <- a (C gy + q).
+// Five of the forward's six slots for each state: 121 us at
+// 1 x 16384 x 2048 x 16 beside the forward's 170, where 32 workgroups of 256
+// CUs alone would work on it in one piece.
 // ---------------------------------------------------------------------------
 struct ScanChunkArgs {
   ScanArgs s;
@@ -651,6 +673,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanFwdArgs f) {
 // LDS as y does; sums over the channels are butterflies over the lanes that
 // halve the number of values at each level and leave one (token, state) in
 // each lane: 63 folds for the 64 values of a wave's round.
+// 23 issue slots for each state and token, of which the formulas are 13 and the
+// folds six. One workgroup a CU and up to 200 registers, with the LDS values of the
+// next eight tokens under way: 16 x 2048 x 2048 x 16 takes 910 us, two
+// workgroups with 128 registers 950. Between two tiles there are two barriers:
+// before the first a thread has the next tile's steps ready, so that between
+// them it only adds, stores and puts. No load waits behind a store: 8 x 2048 x
+// 2048 x 16 took 540 us with a third barrier and loads that did.
 // ---------------------------------------------------------------------------
 struct ScanBwdArgs {
   ScanArgs s;
@@ -973,7 +1002,8 @@ __global__ __launch_bounds__(kScanThreads, 2) void scan_bwd_kernel(ScanBwdArgs f
   }
 }
 
-// gB, gC [B, L, G, N] from the blocks' parts, four states a lane.
+// gB, gC [B, L, G, N] from the blocks' parts, four states a lane: 12.5 us for
+// the 67 MB of 8 x 2048 x 2048 x 16 (5.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_reduce_kernel(ScanArgs a, const float* __restrict__ part,
                                                              T* __restrict__ gb, T* __restrict__ gc) {
@@ -1000,6 +1030,8 @@ __global__ __launch_bounds__(256) void scan_bc_reduce_kernel(ScanArgs a, const f
 
 // One token of each of B sequences, states of a pool updated in place. PER
 // lanes share a channel, four states each. slots as in the convolution's step.
+// Bound by the states, read and written once: 29 us for the 141 MB of 256 x
+// 4096 x 16 (4.9 TB/s; a copy of them 27).
 template <typename T, int PER, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(
     const T* __restrict__ x, const T* __restrict__ dt, const float* __restrict__ A,
