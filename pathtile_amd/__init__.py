@@ -9,6 +9,9 @@ behind the reference's Python surface:
   model and its ``TRAIN_CONV_BACKEND`` switch;
 * ``pathtile_amd.s4convd``                    the S4ConvD model, with each
   block's skip term fused into its convolution;
+* ``pathtile_amd.selective``                  the selective state space block's
+  operators (causal convolution, scan, gated and residual norm), and
+  ``pathtile_amd.selective_model``, a small language model of them;
 * ``pathtile_amd.tune``                       the PathTile offline tuner and
   its selector baselines;
 * ``pathtile_amd.profiling``                  rocprofv3 result summaries.

@@ -41,10 +41,12 @@ static int check_scan(const pt_scan_inputs* in, int L) {
   return in->x && in->dt && in->a && in->b && in->c ? PT_OK : PT_ERR_NULL;
 }
 
-// Tiles of a chunk. A workgroup a CU keeps the chip busy from about 160 on (in
-// one piece 192 take 192 us and 128 take 189 at 2048 tokens of 16 states, in
-// chunks 225 and 160); fewer are cut into chunks of four tiles or more, two to
-// each of 256 CUs, which costs the pass for their states.
+// Tiles of a chunk. A workgroup a CU keeps the chip busy from about 160 on: at
+// 2048 tokens of 16 states 160 take 197 us forward and 448 backward in one
+// piece, 215 and 419 in chunks. Fewer are cut into chunks of four tiles or more,
+// up to 512, which costs the pass for their states: 128 take 154 us forward so
+// (178 with chunks to 256 workgroups, 157 to 1024), and in one piece as long as
+// 160.
 static int scan_chunk_tiles(long long blocks, int ntiles) {
   long long chunks = blocks < 1 || blocks >= 160 ? 1 : ssm_ceil(512, blocks);
   if (chunks > ntiles / 4) chunks = ntiles / 4;

@@ -373,7 +373,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     ``lengths`` [B] (default: L) counts each sequence's tokens: past them y is
     0 and the state stays. With ``return_state`` the result is ``(y, state)``.
     For gradients the forward keeps the states before every 16 tokens (N / 4
-    bytes for each value of x)."""
+    bytes for each value of x, N rounded up to 16) and B and C in FP32."""
     _activation(x, 3, "[B,L,H]")
     x, dt, A, B, C, D, dt_bias = _check_scan(x, dt, A, B, C, D, dt_bias)
     if state is not None:
