@@ -16,7 +16,6 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 using f4v = __attribute__((ext_vector_type(4))) float;
 using u4v = __attribute__((ext_vector_type(4))) uint32_t;
-using u2v = __attribute__((ext_vector_type(2))) uint32_t;
 
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -30,50 +29,29 @@ __device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
 
-// V consecutive values, p aligned to all of them (to 16 bytes from there on).
-template <int V>
-__device__ __forceinline__ void load_vec(const float* p, float (&v)[V]) {
-  static_assert(V % 4 == 0, "whole pieces of 16 bytes");
+// Eight consecutive values, p aligned to 16 bytes.
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < V; i += 4) {
+  for (int i = 0; i < 8; i += 4) {
     const f4v q = *reinterpret_cast<const f4v*>(p + i);
     v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
   }
 }
-template <int V>
-__device__ __forceinline__ void load_vec(const __bf16* p, float (&v)[V]) {
-  static_assert(V == 4 || V % 8 == 0, "8 bytes or whole pieces of 16");
-  if constexpr (V == 4) {
-    const u2v q = *reinterpret_cast<const u2v*>(p);
-    v[0] = bf16_lo(q.x), v[1] = bf16_hi(q.x), v[2] = bf16_lo(q.y), v[3] = bf16_hi(q.y);
-  } else {
+__device__ __forceinline__ void load_vec(const __bf16* p, float (&v)[8]) {
+  const u4v q = *reinterpret_cast<const u4v*>(p);
 #pragma unroll
-    for (int i = 0; i < V; i += 8) {
-      const u4v q = *reinterpret_cast<const u4v*>(p + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + 2 * j] = bf16_lo(q[j]), v[i + 2 * j + 1] = bf16_hi(q[j]);
-    }
-  }
+  for (int j = 0; j < 4; ++j) v[2 * j] = bf16_lo(q[j]), v[2 * j + 1] = bf16_hi(q[j]);
 }
-template <int V>
-__device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < V; i += 4)
+  for (int i = 0; i < 8; i += 4)
     *reinterpret_cast<f4v*>(p + i) = f4v{v[i], v[i + 1], v[i + 2], v[i + 3]};
 }
-template <int V>
-__device__ __forceinline__ void store_vec(__bf16* p, const float (&v)[V]) {
-  if constexpr (V == 4) {
-    *reinterpret_cast<u2v*>(p) = u2v{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
-  } else {
+__device__ __forceinline__ void store_vec(__bf16* p, const float (&v)[8]) {
+  u4v q;
 #pragma unroll
-    for (int i = 0; i < V; i += 8) {
-      u4v q;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = bf16_pair(v[i + 2 * j], v[i + 2 * j + 1]);
-      *reinterpret_cast<u4v*>(p + i) = q;
-    }
-  }
+  for (int j = 0; j < 4; ++j) q[j] = bf16_pair(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<u4v*>(p) = q;
 }
 
 // exp(v). The exponent is rounded once, to 2^-24 |v| of the result; a result

@@ -52,7 +52,7 @@ __device__ __forceinline__ void norm_load(const T* p, int l, int n, float (&v)[E
     for (int i = 0; i < E; i += 8) {
       float q[8] = {};
       const int c = norm_col<E, TPR, VEC>(l, i);
-      if (c < n) load_vec<8>(p + c, q);
+      if (c < n) load_vec(p + c, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i + j] = q[j];
     }
@@ -110,7 +110,7 @@ __device__ __forceinline__ void norm_store(T* p, int l, int n, const float (&v)[
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[j] = v[i + j];
       const int c = norm_col<E, TPR, VEC>(l, i);
-      if (c < n) store_vec<8>(p + c, q);
+      if (c < n) store_vec(p + c, q);
     }
   } else {
 #pragma unroll
