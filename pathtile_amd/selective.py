@@ -23,6 +23,7 @@ Nothing falls back to PyTorch: without the native library every call raises.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Any
 
 import torch
@@ -128,7 +129,9 @@ def _asks_gradient(*tensors: torch.Tensor | None) -> bool:
     return False
 
 
+@lru_cache(maxsize=256)
 def _bytes(query: str, *args: Any) -> int:
+    """What a size query answers, a pure function of its arguments."""
     out = ctypes.c_size_t(0)
     _lib.check(getattr(_lib.load(), query)(*args, ctypes.byref(out)), query)
     return int(out.value)
@@ -138,23 +141,32 @@ def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
 
 
-def _form(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.dtype, t.device)
-
-
 def _save(ctx: Any, *tensors: torch.Tensor | None) -> None:
-    ctx.forms = [_form(t) for t in tensors]
+    ctx.forms = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
     ctx.save_for_backward(*tensors)
 
 
-def _saved(ctx: Any) -> list:
+def _saved(ctx: Any) -> tuple:
     """The saved tensors, which a hook may have given back in other strides
     but not in another shape, type or place."""
     got = ctx.saved_tensors
     for t, form in zip(got, ctx.forms):
-        if _form(t) != form:
-            raise RuntimeError(f"saved tensor {form} was unpacked as {_form(t)}")
-    return list(got)
+        if t is not None and (t.shape != form[0] or t.dtype is not form[1] or t.device != form[2]):
+            raise RuntimeError(f"saved tensor {form} was unpacked as {t.shape, t.dtype, t.device}")
+    return got
+
+
+def _once(backward):
+    """A backward without a second order. A small one runs in the autograd
+    engine's thread at about twice the host time of the same lines elsewhere, so
+    the wrapper that refuses a second order is entered only where one is asked
+    for."""
+    refusing = once_differentiable(backward)
+
+    def run(ctx: Any, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 # --- the short causal convolution ------------------------------------------------
@@ -179,7 +191,7 @@ class CausalConv(torch.autograd.Function):
         return (y, out) if return_state else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, gy, gout=None):
         x, weight, bias, state, lengths = _saved(ctx)
         x, weight = _rows(x), weight.contiguous()
@@ -280,7 +292,12 @@ def _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus):
                            x.shape[0], L, H, N, G, softplus)
 
 
-def _scan_sizes(inputs) -> tuple[int, int, int]:
+@lru_cache(maxsize=256)
+def _scan_sizes(dtype: int, B: int, L: int, H: int, N: int, G: int) -> tuple[int, int, int]:
+    """Bytes of the forward's workspace, of what it saves and of the backward's
+    workspace, which depend on sizes alone."""
+    some = ctypes.addressof(ctypes.c_byte())  # asked for, not read
+    inputs = _lib.ScanInputs(some, some, some, some, some, dtype=dtype, B=B, L=L, H=H, N=N, G=G)
     out = [ctypes.c_size_t(0) for _ in range(3)]
     _lib.check(_lib.load().pt_selective_scan_sizes(ctypes.byref(inputs), *map(ctypes.byref, out)),
                "pt_selective_scan_sizes")
@@ -291,7 +308,7 @@ def _scan_forward(x, dt, A, b, c, D, dt_bias, state, lengths, softplus, return_s
     B, L, H = x.shape
     N = b.shape[-1]
     inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus)
-    ws_bytes, saved_bytes, _ = _scan_sizes(inputs)
+    ws_bytes, saved_bytes, _ = _scan_sizes(_TYPES[x.dtype], B, L, H, N, b.shape[-2])
     y = torch.empty(B, L, H, dtype=x.dtype, device=x.device)
     out = torch.empty(B, H, N, dtype=torch.float32, device=x.device) if return_state else None
     saved = (torch.empty(saved_bytes // 4, dtype=torch.float32, device=x.device)
@@ -314,7 +331,7 @@ class SelectiveScan(torch.autograd.Function):
         return (y, out) if return_state else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, gy, gout=None):
         x, dt, A, b, c, D, dt_bias, state, lengths, saved = _saved(ctx)
         x, dt = _near_rows(x), _near_rows(dt)
@@ -324,7 +341,8 @@ class SelectiveScan(torch.autograd.Function):
         gy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if gy is None else gy.contiguous()
         gout = None if gout is None else gout.contiguous()
         inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, ctx.softplus)
-        ws = _workspace(_scan_sizes(inputs)[2], x)
+        G, N = b.shape[-2:]
+        ws = _workspace(_scan_sizes(_TYPES[x.dtype], *x.shape, N, G)[2], x)
         gx, gdt, ga = torch.empty_like(gy), torch.empty_like(gy), torch.empty_like(A)
         gb, gc = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (b, c))
         gd, gbias = (None if t is None else torch.empty_like(t) for t in (D, dt_bias))
@@ -449,7 +467,7 @@ class GatedNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, gy):
         x, gate, weight, rstd = _saved(ctx)
         x, gate, weight, rstd = _rows(x), _rows(gate), weight.contiguous(), rstd.contiguous()
@@ -505,7 +523,7 @@ class ResidualNorm(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx: Any, gy, gout):
         x, residual, weight, post_weight, scale, rstd, rstd_x = _saved(ctx)
         x, residual = _rows(x), None if residual is None else _rows(residual)
