@@ -41,19 +41,35 @@ static int check_scan(const pt_scan_inputs* in, int L) {
   return in->x && in->dt && in->a && in->b && in->c ? PT_OK : PT_ERR_NULL;
 }
 
-// Tiles of a chunk. A workgroup a CU keeps the chip busy from about 160 on: at
-// 2048 tokens of 16 states 160 take 197 us forward and 448 backward in one
-// piece, 215 and 419 in chunks. Fewer are cut into chunks of four tiles or more,
-// up to 512, which costs the pass for their states: 128 take 154 us forward so
-// (178 with chunks to 256 workgroups, 157 to 1024), and in one piece as long as
-// 160.
-static int scan_chunk_tiles(long long blocks, int ntiles) {
-  long long chunks = blocks < 1 || blocks >= 160 ? 1 : ssm_ceil(512, blocks);
-  if (chunks > ntiles / 4) chunks = ntiles / 4;
-  return (int)ssm_ceil(ntiles, chunks > 1 ? chunks : 1);
+// Tiles of a chunk, by what a CU has to do, in tiles: with k workgroups for each
+// of 256 CUs, k (tiles + 2), and in chunks the first pass too, 0.65 of the
+// forward's time and 0.27 of the backward's. The forward and that pass run two
+// workgroups a CU, and one alone is 1.16 times slower than its share of two.
+// Compared are a sequence in one piece and as many chunks, of four tiles or
+// more, as k = 1 to 12 allow. 2048 tokens, 2048 channels, 16 states, BF16, in
+// one piece and so many chunks:
+//   batch 4: forward 181 us, in 4 140; backward in 2 298, in 4 292
+//   batch 5: forward 181 us, in 8 170; backward 424, in 3 375, in 8 363
+//   batch 8: forward 181 us, in 2 264; backward 458, in 2 557
+//   batch 9: backward 853 us, in 2 690, in 8 642
+static int scan_chunk_tiles(long long blocks, int ntiles, bool backward) {
+  auto cost = [&](int tiles) {
+    const long long chunks = ssm_ceil(ntiles, tiles), k = ssm_ceil(blocks * chunks, 256);
+    const double one = tiles + 2, two = (k == 1 ? 1.16 : k) * one;
+    return (backward ? k * one : two) + (chunks > 1 ? (backward ? 0.27 : 0.65) * two : 0.0);
+  };
+  int best = ntiles;
+  for (int k = 1; k <= 12 && blocks > 0; ++k) {
+    long long chunks = 256 * k / blocks;
+    if (chunks > ntiles / 4) chunks = ntiles / 4;
+    if (chunks < 2) continue;
+    const int tiles = (int)ssm_ceil(ntiles, chunks);
+    if (cost(tiles) < cost(best)) best = tiles;
+  }
+  return best;
 }
 
-static ScanArgs scan_args(const pt_scan_inputs* in) {
+static ScanArgs scan_args(const pt_scan_inputs* in, bool backward) {
   ScanArgs a;
   a.x = in->x, a.dt = in->dt, a.bm = in->b, a.cm = in->c;
   a.x_batch = in->x_batch, a.x_row = in->x_row, a.dt_batch = in->dt_batch, a.dt_row = in->dt_row;
@@ -65,7 +81,7 @@ static ScanArgs scan_args(const pt_scan_inputs* in) {
   a.blocks_g = (int)ssm_ceil(a.hg, kScanCh);
   a.np = (int)ssm_ceil(in->N, 16) * 16;
   a.ntiles = (int)ssm_ceil(in->L, kScanTile);
-  a.chunk_tiles = scan_chunk_tiles((long long)a.B * a.blocks_g * a.G, a.ntiles);
+  a.chunk_tiles = scan_chunk_tiles((long long)a.B * a.blocks_g * a.G, a.ntiles, backward);
   a.chunks = (int)ssm_ceil(a.ntiles, a.chunk_tiles);
   return a;
 }
@@ -127,11 +143,11 @@ int pt_selective_scan_sizes(const pt_scan_inputs* in, size_t* fwd_workspace, siz
   if (!in) return PT_ERR_NULL;
   const int st = pt::check_scan(in, in->L);
   if (st != PT_OK) return st;
-  const pt::ScanArgs a = pt::scan_args(in);
+  const pt::ScanArgs a = pt::scan_args(in, false);
   const size_t bc = pt::scan_bc_floats(a);
   if (fwd_workspace) *fwd_workspace = (pt::scan_chunk_floats(a) + bc) * sizeof(float);
   if (saved) *saved = (pt::scan_state_floats(a) + bc) * sizeof(float);
-  if (bwd_workspace) *bwd_workspace = pt::scan_bwd_layout(a).total;
+  if (bwd_workspace) *bwd_workspace = pt::scan_bwd_layout(pt::scan_args(in, true)).total;
   return PT_OK;
 }
 
@@ -142,7 +158,7 @@ int pt_selective_scan_fwd(const pt_scan_inputs* in, void* y, float* state_out, f
   if (st != PT_OK) return st;
   if (in->B == 0) return PT_OK;
   if (!y) return PT_ERR_NULL;
-  const pt::ScanArgs a = pt::scan_args(in);
+  const pt::ScanArgs a = pt::scan_args(in, false);
   float* ws = static_cast<float*>(workspace);
   const size_t need = (pt::scan_chunk_floats(a) + pt::scan_bc_floats(a)) * sizeof(float);
   if (!workspace || workspace_bytes < need) return PT_ERR_WORKSPACE;
@@ -176,7 +192,7 @@ int pt_selective_scan_bwd(const pt_scan_inputs* in, const void* gy, const float*
   if (st != PT_OK) return st;
   if (!ga) return PT_ERR_NULL;
   if (in->B > 0 && (!gy || !saved || !gx || !gdt || !gb || !gc)) return PT_ERR_NULL;
-  pt::ScanArgs a = pt::scan_args(in);
+  pt::ScanArgs a = pt::scan_args(in, true);
   const pt::ScanBwdLayout o = pt::scan_bwd_layout(a);
   if (in->B > 0 && (!workspace || workspace_bytes < o.total)) return PT_ERR_WORKSPACE;
   if (!pt::ssm_aligned(workspace, 64) || !pt::ssm_aligned(saved, 64)) return PT_ERR_ALIGN;
