@@ -440,7 +440,8 @@ int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* 
  * x, dt [B, L, H]; B, C [B, L, G, N] with contiguous states (b_group: between
  * groups); A [H, N]; D and dt_bias [H] or NULL (0); the first state [B, H, N]
  * or NULL (0). H and the row strides of x and dt are below 2^25.
- * _sizes gives the bytes of the workspaces and of `saved`, which _fwd fills
+ * _sizes gives the bytes of the workspaces (they depend on sizes and on whether
+ * there are lengths) and of `saved`, which _fwd fills
  * where not NULL (the state before every 16 tokens, and B and C in the order
  * that the kernels read) and _bwd takes with the same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;
  * gd, gdt_bias and gstate are skipped where NULL; gb, gc are [B, L, G, N].

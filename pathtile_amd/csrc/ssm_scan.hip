@@ -52,19 +52,24 @@ static int check_scan(const pt_scan_inputs* in, int L) {
 //   batch 5: forward 181 us, in 8 170; backward 424, in 3 375, in 8 363
 //   batch 8: forward 181 us, in 2 264; backward 458, in 2 557
 //   batch 9: backward 853 us, in 2 690, in 8 642
-static int scan_chunk_tiles(long long blocks, int ntiles, bool backward) {
+// With lengths, which the host does not know, workgroups without tokens make
+// room: if fewer than 256 are in one piece, k = 3. Lengths uniform up to 2048, a
+// batch of 5: forward 147 us for 185 by the cost, backward 295 for 348; of 8,
+// which is 256 workgroups, forward 189 for 151, backward 364 for 366.
+static int scan_chunk_tiles(long long blocks, int ntiles, bool backward, bool ragged) {
   auto cost = [&](int tiles) {
     const long long chunks = ssm_ceil(ntiles, tiles), k = ssm_ceil(blocks * chunks, 256);
     const double one = tiles + 2, two = (k == 1 ? 1.16 : k) * one;
     return (backward ? k * one : two) + (chunks > 1 ? (backward ? 0.27 : 0.65) * two : 0.0);
   };
   int best = ntiles;
-  for (int k = 1; k <= 12 && blocks > 0; ++k) {
+  const bool fixed = ragged && blocks < 256;
+  for (int k = fixed ? 3 : 1; k <= (fixed ? 3 : 12) && blocks > 0; ++k) {
     long long chunks = 256 * k / blocks;
     if (chunks > ntiles / 4) chunks = ntiles / 4;
     if (chunks < 2) continue;
     const int tiles = (int)ssm_ceil(ntiles, chunks);
-    if (cost(tiles) < cost(best)) best = tiles;
+    if (fixed || cost(tiles) < cost(best)) best = tiles;
   }
   return best;
 }
@@ -81,7 +86,7 @@ static ScanArgs scan_args(const pt_scan_inputs* in, bool backward) {
   a.blocks_g = (int)ssm_ceil(a.hg, kScanCh);
   a.np = (int)ssm_ceil(in->N, 16) * 16;
   a.ntiles = (int)ssm_ceil(in->L, kScanTile);
-  a.chunk_tiles = scan_chunk_tiles((long long)a.B * a.blocks_g * a.G, a.ntiles, backward);
+  a.chunk_tiles = scan_chunk_tiles((long long)a.B * a.blocks_g * a.G, a.ntiles, backward, a.lengths != nullptr);
   a.chunks = (int)ssm_ceil(a.ntiles, a.chunk_tiles);
   return a;
 }

@@ -293,11 +293,13 @@ def _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus):
 
 
 @lru_cache(maxsize=256)
-def _scan_sizes(dtype: int, B: int, L: int, H: int, N: int, G: int) -> tuple[int, int, int]:
+def _scan_sizes(dtype: int, B: int, L: int, H: int, N: int, G: int,
+                ragged: bool) -> tuple[int, int, int]:
     """Bytes of the forward's workspace, of what it saves and of the backward's
-    workspace, which depend on sizes alone."""
+    workspace, which depend on sizes and on whether there are lengths."""
     some = ctypes.addressof(ctypes.c_byte())  # asked for, not read
-    inputs = _lib.ScanInputs(some, some, some, some, some, dtype=dtype, B=B, L=L, H=H, N=N, G=G)
+    inputs = _lib.ScanInputs(some, some, some, some, some, lengths=some if ragged else None,
+                             dtype=dtype, B=B, L=L, H=H, N=N, G=G)
     out = [ctypes.c_size_t(0) for _ in range(3)]
     _lib.check(_lib.load().pt_selective_scan_sizes(ctypes.byref(inputs), *map(ctypes.byref, out)),
                "pt_selective_scan_sizes")
@@ -308,7 +310,8 @@ def _scan_forward(x, dt, A, b, c, D, dt_bias, state, lengths, softplus, return_s
     B, L, H = x.shape
     N = b.shape[-1]
     inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, softplus)
-    ws_bytes, saved_bytes, _ = _scan_sizes(_TYPES[x.dtype], B, L, H, N, b.shape[-2])
+    ws_bytes, saved_bytes, _ = _scan_sizes(_TYPES[x.dtype], B, L, H, N, b.shape[-2],
+                                           lengths is not None)
     y = torch.empty(B, L, H, dtype=x.dtype, device=x.device)
     out = torch.empty(B, H, N, dtype=torch.float32, device=x.device) if return_state else None
     saved = (torch.empty(saved_bytes // 4, dtype=torch.float32, device=x.device)
@@ -342,7 +345,7 @@ class SelectiveScan(torch.autograd.Function):
         gout = None if gout is None else gout.contiguous()
         inputs = _scan_inputs(x, dt, A, b, c, D, dt_bias, state, lengths, ctx.softplus)
         G, N = b.shape[-2:]
-        ws = _workspace(_scan_sizes(_TYPES[x.dtype], *x.shape, N, G)[2], x)
+        ws = _workspace(_scan_sizes(_TYPES[x.dtype], *x.shape, N, G, lengths is not None)[2], x)
         gx, gdt, ga = torch.empty_like(gy), torch.empty_like(gy), torch.empty_like(A)
         gb, gc = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (b, c))
         gd, gbias = (None if t is None else torch.empty_like(t) for t in (D, dt_bias))
