@@ -441,10 +441,11 @@ int pt_causal_conv_step(int dtype, const void* x, long long x_row, const float* 
  * groups); A [H, N]; D and dt_bias [H] or NULL (0); the first state [B, H, N]
  * or NULL (0). H and the row strides of x and dt are below 2^25.
  * _sizes gives the bytes of the workspaces (they depend on sizes and on whether
- * there are lengths) and of `saved`, which _fwd fills
- * where not NULL (the state before every 16 tokens, and B and C in the order
- * that the kernels read) and _bwd takes with the same inputs. _bwd: gstate_out (NULL: 0) is the final state's gradient;
- * gd, gdt_bias and gstate are skipped where NULL; gb, gc are [B, L, G, N].
+ * there are lengths) and of `saved`, which _fwd fills where not NULL (the state
+ * before every 16 tokens, and B and C in the order that the kernels read) and
+ * _bwd takes with the same inputs. _bwd: gstate_out (NULL: 0) is the final
+ * state's gradient; gd, gdt_bias and gstate are skipped where NULL; gb, gc are
+ * [B, L, G, N].
  * _step: one token, x and dt [B, H] and B, C [B, G, N] with the batch strides
  * (row strides and L are not read); states [pool, H, N] and slots as in
  * pt_causal_conv_step.
